@@ -21,6 +21,11 @@ LIB_PATH = os.path.join(HERE, "libbagel_hip.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "bagel_hip.h")
 SOURCES = ["capi.hip", "gemm.hip", "skinny.hip", "attention.hip", "elementwise.hip", "vae.hip", "layer.hip", "decode_attention.hip"]
 
+# Packed fp32 arithmetic is kept out of the generated code: some forms of v_pk_{add,mul,fma}_f32 are not reliable here,
+# and the compiler makes them from ordinary scalar float code.
+HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value",
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -28,8 +33,8 @@ STAMP_PATH = LIB_PATH + ".sha256"   # travels with the library
 
 
 def source_digest() -> str:
-    """SHA-256 over every file the library is compiled from (csrc/*.hip, csrc/*.h, the public header)."""
-    h = hashlib.sha256()
+    """SHA-256 over every file the library is compiled from (csrc/*.hip, csrc/*.h, the public header) and the flags."""
+    h = hashlib.sha256(" ".join(HIPCC_FLAGS).encode())
     for path in sorted(glob.glob(os.path.join(CSRC, "*.hip")) + glob.glob(os.path.join(CSRC, "*.h"))) + [HEADER]:
         h.update(os.path.basename(path).encode())
         with open(path, "rb") as f:
@@ -53,7 +58,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     for s in srcs:
         o = os.path.join(HERE, "build", os.path.basename(s) + ".o")
         objs.append(o)
-        cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-c", s, "-o", o]
+        cmd = [hipcc, *HIPCC_FLAGS, "-c", s, "-o", o]
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     for cmd, pr in procs:
         out, _ = pr.communicate()

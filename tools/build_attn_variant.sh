@@ -5,6 +5,7 @@ set -e
 ROOT="$(cd "$(dirname "$0")/.." && pwd)"
 name="$1"; shift
 mkdir -p "$ROOT/tools/_ab"
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-value "$@" -shared \
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-value \
+  -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -shared \
   "$ROOT/bagel_amd/csrc/attention.hip" "$ROOT/bagel_amd/csrc/capi.hip" -o "$ROOT/tools/_ab/libattn_$name.so"
 echo "$ROOT/tools/_ab/libattn_$name.so"

@@ -17,7 +17,7 @@ def main():
     for s in _lib.SOURCES:
         o = os.path.join(out_dir, "obj_" + name, s + ".o")
         objs.append(o)
-        cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", *flags, "-c",
+        cmd = ["/opt/rocm/bin/hipcc", *_lib.HIPCC_FLAGS, *flags, "-c",
                os.path.join(_lib.CSRC, s), "-o", o]
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     for cmd, p in procs:
