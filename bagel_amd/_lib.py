@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import glob
 import hashlib
+import math
 import os
 import re
 import subprocess
@@ -19,7 +20,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libbagel_hip.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "bagel_hip.h")
-SOURCES = ["capi.hip", "gemm.hip", "skinny.hip", "attention.hip", "elementwise.hip", "vae.hip", "layer.hip", "decode_attention.hip"]
+SOURCES = ["capi.hip", "gemm.hip", "skinny.hip", "attention.hip", "elementwise.hip", "vae.hip", "layer.hip", "decode_attention.hip", "paged.hip"]
 
 # Packed fp32 arithmetic is kept out of the generated code: some forms of v_pk_{add,mul,fma}_f32 are not reliable here,
 # and the compiler makes them from ordinary scalar float code.
@@ -97,7 +98,7 @@ def lib() -> ctypes.CDLL:
         _lib = ctypes.CDLL(variant if variant else LIB_PATH)
         _lib.bagel_last_error.restype = ctypes.c_char_p
         for name in ("bagel_skinny_gemm_workspace_bytes", "bagel_cfg_workspace_bytes", "bagel_groupnorm_workspace_bytes",
-                     "bagel_decode_attention_workspace_bytes"):
+                     "bagel_decode_attention_workspace_bytes", "bagel_paged_decode_attention_workspace_bytes"):
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = ctypes.c_long
     return _lib
@@ -359,6 +360,142 @@ def decode_attention(qkv, Hq, Hkv, D, q_norm, k_norm, cos_t, sin_t, row_cs, row_
                                              _p(Vt_ws), L(S), _p(O), F(eps), I(1 if und_rounding else 0), L(max_kv_len), _p(workspace),
                                              L(workspace.numel() * workspace.element_size()), _stream()),
            "bagel_decode_attention_bf16")
+
+
+# ---- a paged key-value cache ---------------------------------------------------------------------
+# The calls of a serving loop are short on the device, so what can be checked once is checked when a PagedCache is made,
+# and the argument types are declared to ctypes instead of being wrapped per call.
+E4M3 = torch.float8_e4m3fn
+
+
+def _require(ok, message):
+    if not ok:
+        raise RuntimeError(message)
+
+
+def _here(*tensors):
+    """Addresses of tensors (None: 0) that must live on the current device."""
+    for t in tensors:
+        _require(t is None or t.is_cuda, "device tensor expected")
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            _p(t)      # raises, and names both devices
+    return [0 if t is None else t.data_ptr() for t in tensors]
+
+
+def _rows(t, width, name):
+    """Row stride of a [rows, ...] bf16 tensor whose rows are ``width`` contiguous elements."""
+    n = 1
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        _require(size == 1 or stride == n, f"{name}: the elements of a row must be contiguous")
+        n *= size
+    _require(t.dtype == torch.bfloat16 and n == width, f"{name}: {t.dtype} rows of {n} elements, bfloat16 rows of {width} expected")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+
+
+def _ints(t, shape, name):
+    _require(t.dtype == torch.int32 and t.shape == shape and t.is_contiguous(),
+             f"{name}: contiguous int32 {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}")
+
+
+class _PagedCacheStruct(ctypes.Structure):
+    _fields_ = [("k", VP), ("v", VP)] + [(f"{x}_{s}_stride", L) for x in "kv" for s in ("page", "slot", "head")] + \
+               [(n, I) for n in ("num_pages", "page_size", "num_kv_heads", "head_dim", "e4m3")] + [("k_scale", VP), ("v_scale", VP)]
+
+
+class PagedCache:
+    """One layer's pool of pages (bagel_paged_cache): ``k_pages`` / ``v_pages`` are ``[pages, slots, kv heads, head_dim]``
+    views of any memory order with contiguous head rows (``pool.transpose(1, 2)`` of a heads-first pool, ``kv[:, 0]`` of a
+    joint one), bfloat16 or, with fp32 ``k_scale`` / ``v_scale`` ``[kv heads]``, float8_e4m3fn.  It holds the tensors and is
+    the argument of paged_kv_append and paged_decode_attention."""
+
+    def __init__(self, k_pages, v_pages, k_scale=None, v_scale=None):
+        _require(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and min(k_pages.shape) > 0,
+                 f"paged cache: two pools [pages, slots, kv heads, head_dim] expected, got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+        _require(k_pages.dtype == v_pages.dtype and k_pages.dtype in (torch.bfloat16, E4M3),
+                 f"paged cache: bfloat16 or float8_e4m3fn pools expected, got {k_pages.dtype} and {v_pages.dtype}")
+        self.pages, self.page_size, self.heads, self.head_dim = k_pages.shape
+        self.e4m3 = k_pages.dtype == E4M3
+        for t in (k_pages, v_pages):
+            _require(t.stride(3) == 1, "paged cache: the head_dim elements must be contiguous")
+        for t in (k_scale, v_scale):
+            _require((t is not None) == self.e4m3, "paged cache: k_scale and v_scale belong to a float8_e4m3fn cache, both of them")
+            _require(t is None or (t.dtype == torch.float32 and t.shape == (self.heads,) and t.is_contiguous()),
+                     f"paged cache: scales are contiguous float32 [{self.heads}]")
+        self.k_pages, self.v_pages, self.k_scale, self.v_scale = k_pages, v_pages, k_scale, v_scale
+        held = [t for t in (k_pages, v_pages, k_scale, v_scale) if t is not None]
+        _require(all(t.device == k_pages.device for t in held), "paged cache: pools and scales on different devices")
+        addr = [0 if t is None else t.data_ptr() for t in (k_pages, v_pages, k_scale, v_scale)]
+        # a dimension of one element has no stride of its own
+        strides = [t.stride(d) if t.shape[d] > 1 else self.head_dim for t in (k_pages, v_pages) for d in range(3)]
+        self.struct = _PagedCacheStruct(addr[0], addr[1], *strides, self.pages, self.page_size, self.heads, self.head_dim,
+                                        int(self.e4m3), addr[2] or None, addr[3] or None)
+        self.ref = ctypes.byref(self.struct)
+
+
+def _declared(name, *types):
+    fn = getattr(lib(), name)
+    if fn.argtypes is None:
+        fn.argtypes = types
+    return fn
+
+
+def paged_kv_append(qkv, Hq, cache: PagedCache, row_slot, Q=None, q_norm=None, k_norm=None, cos_t=None, sin_t=None, row_cs=None,
+                    eps=1e-6, und_rounding=False):
+    """q/k norm + RoPE of qkv's rows; keys and values to the cache's slots ``row_slot`` (negative: padding, left alone), the
+    queries to ``Q`` [rows, Hq, head_dim] (bagel_paged_kv_append_bf16).  No norm weight: no norm; no tables: no rotation."""
+    rows, D = qkv.shape[0], cache.head_dim
+    _require(Hq >= 0 and (Hq > 0 or Q is None), "paged_kv_append: Q without query heads")
+    ld = _rows(qkv, (Hq + 2 * cache.heads) * D, "paged_kv_append: qkv")
+    _ints(row_slot, (rows,), "paged_kv_append: row_slot")
+    ldq = 0
+    if Q is not None:
+        _require(Q.shape[0] == rows, f"paged_kv_append: Q has {Q.shape[0]} rows, qkv {rows}")
+        ldq = _rows(Q, Hq * D, "paged_kv_append: Q")
+    for w in (q_norm, k_norm):
+        _require(w is None or (w.dtype == torch.bfloat16 and w.shape == (D,) and w.is_contiguous()),
+                 f"paged_kv_append: norm weights are contiguous bfloat16 [{D}]")
+    _require((cos_t is None) == (sin_t is None) == (row_cs is None), "paged_kv_append: cos_t, sin_t and row_cs come together")
+    if cos_t is not None:
+        _require(cos_t.dtype == sin_t.dtype == torch.bfloat16 and cos_t.dim() == 2 and cos_t.shape[1] == D and
+                 cos_t.shape == sin_t.shape and cos_t.is_contiguous() and sin_t.is_contiguous(),
+                 f"paged_kv_append: rotation tables are contiguous bfloat16 [positions, {D}]")
+        _ints(row_cs, (rows,), "paged_kv_append: row_cs")
+    a = _here(qkv, row_slot, Q, q_norm, k_norm, cos_t, sin_t, row_cs, cache.k_pages)
+    fn = _declared("bagel_paged_kv_append_bf16", VP, L, I, I, VP, VP, VP, VP, VP, I, VP, VP, VP, L, F, I, VP)
+    _check(fn(a[0], ld, rows, Hq, cache.ref, a[3], a[4], a[5], a[6], 0 if cos_t is None else cos_t.shape[0], a[7], a[1], a[2], ldq,
+              eps, 1 if und_rounding else 0, _stream()), "bagel_paged_kv_append_bf16")
+    return Q
+
+
+def paged_decode_attention_workspace_bytes(rows, Hq, Hkv, D, max_kv_len) -> int:
+    return int(lib().bagel_paged_decode_attention_workspace_bytes(I(rows), I(Hq), I(Hkv), I(D), L(max_kv_len)))
+
+
+def paged_decode_attention(Q, cache: PagedCache, page_table, kv_lens, O, workspace, max_kv_len=0, softmax_scale=None):
+    """Attention of one new token per row over its first ``kv_lens[row]`` cached keys (bagel_paged_decode_attention_bf16):
+    Q, O [rows, Hq, head_dim]; page_table [rows, pages] int32; workspace: paged_decode_attention_workspace_bytes, made with
+    torch.zeros; max_kv_len: an upper bound of kv_lens known on the host (0: the table's width)."""
+    D = cache.head_dim
+    _require(Q.dim() == 3 and Q.shape == O.shape and Q.shape[2] == D and Q.shape[1] > 0 and Q.shape[1] % cache.heads == 0,
+             f"paged_decode_attention: Q {tuple(Q.shape)} and O {tuple(O.shape)} must be [rows, a multiple of {cache.heads} heads, {D}]")
+    rows, Hq = Q.shape[0], Q.shape[1]
+    ldq, ldo = _rows(Q, Hq * D, "paged_decode_attention: Q"), _rows(O, Hq * D, "paged_decode_attention: O")
+    _require(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == rows and page_table.shape[1] > 0 and
+             page_table.stride(1) == 1, f"paged_decode_attention: page_table must be int32 [{rows}, pages] with contiguous rows")
+    _ints(kv_lens, (rows,), "paged_decode_attention: kv_lens")
+    _require(max_kv_len >= 0, "paged_decode_attention: max_kv_len is negative")
+    _require(softmax_scale is None or (softmax_scale != 0 and math.isfinite(softmax_scale)),
+             f"paged_decode_attention: softmax_scale {softmax_scale}")
+    _require(workspace.is_contiguous(), "paged_decode_attention: contiguous workspace expected")
+    a = _here(Q, page_table, kv_lens, O, workspace, cache.k_pages)
+    width = page_table.shape[1]
+    fn = _declared("bagel_paged_decode_attention_bf16", VP, L, I, I, VP, VP, L, I, VP, L, VP, L, F, VP, L, VP)
+    _check(fn(a[0], ldq, rows, Hq, cache.ref, a[1], page_table.stride(0) if rows > 1 else width, width, a[2], max_kv_len, a[3], ldo,
+              softmax_scale or 0.0, a[4], workspace.numel() * workspace.element_size(), _stream()),
+           "bagel_paged_decode_attention_bf16")
+    return O
 
 
 def mot_forward(dims: MotDims, layers, n_layers, rows: MotRows, K_ws, Vt_ws, kv_only_last=False, final_norm_gen=None,

@@ -1,0 +1,547 @@
+// A paged key-value cache (gfx950): append of new keys and values with the q/k norm and the rotation on the way, and one
+// new token's attention over it.
+//
+// The cache is a pool of pages of page_size slots, element (page, slot, kv head, d) at
+// page * page_stride + slot * slot_stride + head * head_stride + d, in bf16 or in OCP e4m3 with one fp32 scale per kv
+// head (a stored unit stands for `scale`).  A sequence owns pages in any order; its page table row lists them.  Rows of a
+// head are contiguous, whichever of slots and heads comes first, and nothing about a sequence's length or place is fixed:
+// sequences grow page by page, finish and hand their pages on without a copy.
+#include "common.h"
+#include <algorithm>
+#include "qk_rope.h"
+#include "../../include/bagel_hip.h"
+
+namespace {
+
+constexpr float E4M3_MAX = 448.f;
+
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
+
+struct Pool {          // one of the two pools, strides in BYTES
+  char* base;
+  long page, slot, head;
+  const float* scale;  // per kv head, null for bf16
+};
+
+// fp32 -> four e4m3 in a dword, round to nearest even, clamped to the largest finite value (a NaN stays one: the clamp is
+// written so that it passes).
+__device__ __forceinline__ unsigned pack_e4m3(float a, float b, float c, float d) {
+  auto clamp = [](float x) { return x > E4M3_MAX ? E4M3_MAX : x < -E4M3_MAX ? -E4M3_MAX : x; };
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(clamp(a), clamp(b), 0, false);
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(clamp(c), clamp(d), r, true);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Append.  Row r of qkv holds Hq query heads, Hkv key heads and Hkv value heads of D; D / 8 lanes hold a head (16 bytes
+// each), so a head's norm and its rotation partner stay inside those lanes.  Everything is one pass: each projected
+// element is read once and each result written once.
+// ---------------------------------------------------------------------------------------------------------------------
+struct AppendParams {
+  const bf16* qkv;
+  long ld;
+  const bf16 *q_w, *k_w, *cos_t, *sin_t;   // norm weights [D], rotation rows [*][D]; null: that step is left out
+  const int *row_cs, *row_slot;
+  bf16* Q;                                 // null: queries are not asked for
+  long ldq;
+  Pool k, v;
+  long capacity;                           // slots in the pool
+  int rows, Hq, Hkv, page_shift, cs_rows, und_rounding;
+  float eps;
+};
+
+template <int D, bool F8>
+__global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
+  constexpr int LPH = D / 8;
+  const int heads = p.Hq + 2 * p.Hkv;
+  const long item = ((long)blockIdx.x * 256 + threadIdx.x) / LPH;
+  if (item >= (long)p.rows * heads) return;      // a head's lanes leave together
+  const int j = threadIdx.x % LPH;
+  const int row = (int)(item / heads), head = (int)(item % heads);
+  const int slot = p.row_slot[row];
+  if (slot < 0) return;                          // padding: the cache and the row's queries are left as they are
+  const bool is_q = head < p.Hq, is_v = head >= p.Hq + p.Hkv;
+  if (is_q && !p.Q) return;
+  const int cs = p.cos_t ? p.row_cs[row] : 0;
+  bf16x8 x = *(const bf16x8*)(p.qkv + row * p.ld + (long)head * D + 8 * j);
+  if (slot >= p.capacity || (p.cos_t && (cs < 0 || cs >= p.cs_rows))) {
+    // a slot or rotation row that does not exist: nothing is stored, and the row's queries say so
+    if (is_q) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (bf16)__builtin_nanf("");
+      *(bf16x8*)(p.Q + row * p.ldq + (long)head * D + 8 * j) = x;
+    }
+    return;
+  }
+  float y[8];
+  if (is_v) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (float)x[e];
+  } else {
+    norm_rope_lane<D>(x, j, is_q ? p.q_w : p.k_w, p.cos_t ? p.cos_t + (long)cs * D : nullptr,
+                      p.cos_t ? p.sin_t + (long)cs * D : nullptr, p.eps, p.und_rounding, y);
+  }
+  bf16x8 o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = (bf16)y[e];
+  if (is_q) {
+    *(bf16x8*)(p.Q + row * p.ldq + (long)head * D + 8 * j) = o;
+    return;
+  }
+  const Pool& pool = is_v ? p.v : p.k;
+  const int h = head - p.Hq - (is_v ? p.Hkv : 0);
+  char* dst = pool.base + (long)(slot >> p.page_shift) * pool.page + (long)(slot & ((1 << p.page_shift) - 1)) * pool.slot + h * pool.head;
+  if constexpr (F8) {
+    const float s = pool.scale[h];
+    *(u32x2*)(dst + 8 * j) = u32x2{pack_e4m3(y[0] / s, y[1] / s, y[2] / s, y[3] / s), pack_e4m3(y[4] / s, y[5] / s, y[6] / s, y[7] / s)};
+  } else {
+    *(bf16x8*)(dst + 16 * j) = o;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Attention of one new token per row.
+//
+// The keys and values of a (row, kv head) are read once for all the query heads that share them, up to 16 per workgroup,
+// so that the matrix instruction's 16 columns are heads:
+//   S^T[key][head] = K . Q^T      and      O^T[d][head] += V^T . P^T
+// with 32 keys as the contraction of the second product.  Nothing passes through LDS on the way:
+//   - A lane of S^T's operand holds 16 bytes of ONE key row (lane & 15 = row, lane >> 4 = part of the contraction).
+//   - Row m of key tile t is key 8 (m / 4) + 4 t + m % 4 of the 32, so that the results a lane gets - rows 4 g + i of both
+//     tiles, g = lane >> 4 - are keys 8 g ... 8 g + 7 of its head: exactly what the second product wants of P^T from it.
+//   - V rows are read whole (16 lanes x D / 16 elements, 8 keys per lane group).  The operand wants 8 KEYS of one d per
+//     lane; the lane has D / 16 d's of those 8 keys, so byte permutes turn one into the other inside the lane, and
+//     row r of product dd is d = (D / 16) r + dd.
+// The softmax is the running form: one maximum and sum per head and wave, scores and sums in fp32, P rounded to bf16 for
+// the matrix product (an error of 2^-9 of each weight, which the output's own rounding to bf16 exceeds).
+// An e4m3 value is a bf16 value: keys and values are widened exactly, the scales enter in fp32.
+//
+// One workgroup = four waves that take turns at the chunk's tiles, each with its own running softmax; two tiles of every
+// wave are in flight while it computes.  A row with more keys than one chunk is split over workgroups; each leaves an
+// unnormalised partial (sums in fp32) and the last one to finish joins them in chunk order.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int WAVES = 4;
+constexpr int MAX_SPLITS = 128;
+
+struct AttendParams {
+  const bf16* Q;
+  long ldq;
+  Pool k, v;
+  const int* table;      // [rows][table_width] page ids
+  long table_stride;
+  int table_width, num_pages, page_shift;
+  const int* kv_lens;
+  bf16* O;
+  long ldo;
+  float* part;           // [rows][Hkv][head blocks][splits][heads in the block][D + 2]
+  unsigned* tickets;     // [rows][Hkv][head blocks], zero on entry, left zero
+  int Hq, Hkv, chunk;
+  float scale_log2;
+};
+
+__device__ __forceinline__ bf16x8 widen8(unsigned a, unsigned b) {   // eight e4m3 -> eight bf16
+  const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false), x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+  const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false), x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+  return bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+}
+
+// maximum / sum over the four lanes that hold one head's column
+__device__ __forceinline__ float column_max(float v) {
+  const u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const u32x2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  const u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const u32x2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+template <int D, bool F8>
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_attention_kernel(AttendParams p) {
+  constexpr int ITEM = F8 ? 1 : 2;
+  constexpr int SUB = 256 / (D * ITEM);        // blocks of 32 keys per tile: a tile is 8 KB of keys and 8 KB of values
+  constexpr int TK = 32 * SUB;                 // keys per tile
+  constexpr int KC = D * ITEM / 64;            // 16-byte loads of a key row per lane
+  constexpr int KM = D / 32;                   // matrix instructions per 16 keys of S^T
+  constexpr int ND = D / 16;                   // d's per lane of a value row
+  constexpr int VW = ND * ITEM / 4;            // dwords per lane of a value row
+  constexpr int PW = D + 2;                    // floats of a partial: sums, maximum, weight
+  const int row = blockIdx.z, kvh = blockIdx.y % p.Hkv, hb = blockIdx.y / p.Hkv, c = blockIdx.x;
+  const int rep = p.Hq / p.Hkv, h0 = hb * 16, nh = min(16, rep - h0);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  int len = p.kv_lens[row];
+  const long head0 = (long)kvh * rep + h0;     // first query head of this workgroup
+  bf16* orow = p.O + row * p.ldo + head0 * D;
+  if (len <= 0) {                              // a free slot of the batch: zeros
+    if (c == 0)
+      for (int i = tid; i < nh * D / 8; i += 64 * WAVES) *(u32x4*)(orow + 8 * i) = u32x4{0, 0, 0, 0};
+    return;
+  }
+  bool bad = len > p.table_width << p.page_shift;   // more keys than the row's table has pages for
+  if (bad) len = p.table_width << p.page_shift;
+  // at most as many chunks as the grid has: a bound on the lengths that was too small costs time, not keys
+  const int splits_max = (int)gridDim.x;
+  const int chunk = max(p.chunk, ((len + splits_max - 1) / splits_max + TK - 1) / TK * TK);
+  const int nsplit = (len + chunk - 1) / chunk;
+  if (c >= nsplit) return;
+  const int begin = c * chunk, end = min(len - begin, chunk) + begin;
+
+  __shared__ float o_s[WAVES][16][D + 4];
+  __shared__ float m_s[WAVES][16], l_s[WAVES][16];
+  __shared__ unsigned ticket_s;
+
+  const int* table = p.table + row * p.table_stride;
+  const int mask = (1 << p.page_shift) - 1;
+  const int last_page = (len - 1) >> p.page_shift;
+  const int kr = 8 * (n >> 2) + (n & 3);       // this lane's key row (of tile 0) among 32
+  const char* kbase = p.k.base + kvh * p.k.head + 16 * g;
+  const char* vbase = p.v.base + kvh * p.v.head + n * (ND * ITEM);
+
+  struct Ids {
+    int k[SUB], v[SUB];
+  };
+  struct Tile {
+    u32x4 k[SUB][2][KC];
+    unsigned v[SUB][8][VW];
+  };
+  // page ids of the tile at key k0; a page id outside the pool is not followed: the row's output says so instead
+  auto load_ids = [&](Ids& x, int k0) {
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      x.k[s] = table[min((k0 + 32 * s + (kr & ~7)) >> p.page_shift, last_page)];
+      x.v[s] = table[min((k0 + 32 * s + 8 * g) >> p.page_shift, last_page)];
+    }
+  };
+  auto load_tile = [&](Tile& x, const Ids& ids, int k0) {
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      const bool kb = (unsigned)ids.k[s] >= (unsigned)p.num_pages, vb = (unsigned)ids.v[s] >= (unsigned)p.num_pages;
+      bad |= kb | vb;
+      const char* kp = kbase + (long)(kb ? 0 : ids.k[s]) * p.k.page + (long)((k0 + 32 * s + kr) & mask) * p.k.slot;
+      const char* vp = vbase + (long)(vb ? 0 : ids.v[s]) * p.v.page + (long)((k0 + 32 * s + 8 * g) & mask) * p.v.slot;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < KC; ++i) x.k[s][t][i] = *(const u32x4*)(kp + 4 * t * p.k.slot + 64 * i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (VW == 4) {
+          const u32x4 w = *(const u32x4*)(vp + e * p.v.slot);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x.v[s][e][i] = w[i];
+        } else if constexpr (VW == 2) {
+          const u32x2 w = *(const u32x2*)(vp + e * p.v.slot);
+          x.v[s][e][0] = w[0];
+          x.v[s][e][1] = w[1];
+        } else {
+          x.v[s][e][0] = *(const unsigned*)(vp + e * p.v.slot);
+        }
+      }
+    }
+  };
+
+  // queries: column n of the operand is head n; element e of lane group g is d = 32 j + 8 g + e (bf16 keys) or
+  // 64 (j / 2) + 16 g + 8 (j % 2) + e (e4m3: a 16-byte load of keys feeds two instructions)
+  bf16x8 q[KM];
+#pragma unroll
+  for (int j = 0; j < KM; ++j) {
+    const int d = F8 ? 64 * (j / 2) + 16 * g + 8 * (j % 2) : 32 * j + 8 * g;
+    q[j] = *(const bf16x8*)(p.Q + row * p.ldq + (head0 + min(n, nh - 1)) * D + d);
+  }
+  const float scale = p.scale_log2 * (F8 ? p.k.scale[kvh] : 1.0f);
+
+  f32x4 acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY, l_run = 0.f;        // l_run: this lane's keys only
+
+  auto compute = [&](Tile& x, int k0) {
+    float s[SUB][8];
+#pragma unroll
+    for (int b = 0; b < SUB; ++b)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KM; ++j) {
+          bf16x8 kf;
+          if constexpr (F8) {
+            const u32x4 w = x.k[b][t][j / 2];
+            kf = widen8(w[2 * (j % 2)], w[2 * (j % 2) + 1]);
+          } else {
+            kf = __builtin_bit_cast(bf16x8, x.k[b][t][j]);
+          }
+          a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[j], a, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[b][4 * t + i] = a[i] * scale;
+      }
+    if (k0 + TK > end) {
+      // keys behind the end: their scores are replaced, and their values cleared (0 x NaN is NaN)
+#pragma unroll
+      for (int b = 0; b < SUB; ++b)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k0 + 32 * b + 8 * g + e >= end) {
+            s[b][e] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < VW; ++i) x.v[b][e][i] = 0;
+          }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < SUB; ++b)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[b][e]);
+    const float m_new = fmaxf(m_run, column_max(mx));
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+    m_run = m_new;
+    l_run *= alpha;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) acc[i] *= alpha;
+#pragma unroll
+    for (int b = 0; b < SUB; ++b) {
+      bf16x8 pb;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float w = __builtin_amdgcn_exp2f(s[b][e] - m_new);
+        l_run += w;
+        pb[e] = (bf16)w;
+      }
+#pragma unroll
+      for (int dd = 0; dd < ND; ++dd) {
+        u32x4 a;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (F8) {
+            const unsigned w = __builtin_amdgcn_perm(x.v[b][2 * i + 1][dd / 4], x.v[b][2 * i][dd / 4], dd % 4 < 2 ? 0x05010400u : 0x07030602u);
+            const bf16x2 two = dd % 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
+                                      : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+            a[i] = __builtin_bit_cast(unsigned, two);
+          } else {
+            a[i] = __builtin_amdgcn_perm(x.v[b][2 * i + 1][dd / 2], x.v[b][2 * i][dd / 2], dd % 2 ? 0x07060302u : 0x05040100u);
+          }
+        }
+        acc[dd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), pb, acc[dd], 0, 0, 0);
+      }
+    }
+  };
+
+  Ids ia, ib;
+  Tile ta, tb;
+  constexpr int STEP = WAVES * TK;
+  int k0 = begin + wave * TK;
+  if (k0 < end) load_ids(ia, k0);
+  if (k0 + STEP < end) load_ids(ib, k0 + STEP);
+  if (k0 < end) load_tile(ta, ia, k0);
+  if (k0 + 2 * STEP < end) load_ids(ia, k0 + 2 * STEP);
+  if (k0 + STEP < end) load_tile(tb, ib, k0 + STEP);
+  if (k0 + 3 * STEP < end) load_ids(ib, k0 + 3 * STEP);
+  for (; k0 < end; k0 += 2 * STEP) {
+    compute(ta, k0);
+    if (k0 + 2 * STEP < end) load_tile(ta, ia, k0 + 2 * STEP);
+    if (k0 + 4 * STEP < end) load_ids(ia, k0 + 4 * STEP);
+    if (k0 + STEP < end) compute(tb, k0 + STEP);
+    if (k0 + 3 * STEP < end) load_tile(tb, ib, k0 + 3 * STEP);
+    if (k0 + 5 * STEP < end) load_ids(ib, k0 + 5 * STEP);
+  }
+
+  // ---- join the waves
+  l_run = column_sum(l_run);
+  if (__any(bad)) l_run = __builtin_nanf("");
+  if (g == 0) {
+    m_s[wave][n] = m_run;
+    l_s[wave][n] = l_run;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int dd = 0; dd < ND; ++dd) o_s[wave][n][ND * (4 * g + i) + dd] = acc[dd][i];
+  __syncthreads();
+  const float vscale = F8 ? p.v.scale[kvh] : 1.0f;
+  const long pair = ((long)row * p.Hkv + kvh) * ((rep + 15) / 16) + hb;
+  // partials of all head blocks of a (row, kv head) lie together: rep heads of `splits_max` chunks
+  float* part = p.part + (((long)row * p.Hkv + kvh) * rep + h0) * splits_max * PW;
+  for (int i = tid; i < nh * D; i += 64 * WAVES) {
+    const int h = i / D, d = i % D;
+    float mx = m_s[0][h];                                   // wave 0 always had a tile
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) mx = fmaxf(mx, m_s[w][h]);
+    float o = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float f = __builtin_amdgcn_exp2f(m_s[w][h] - mx);
+      o += o_s[w][h][d] * f;
+      l += l_s[w][h] * f;
+    }
+    if (nsplit == 1) {
+      orow[i] = (bf16)(o / l * vscale);
+    } else {
+      // Partials pass between workgroups on different XCDs by the same forms as in decode_attention.hip: agent-scope
+      // stores and loads (written through, read past the CU's cache), every store complete before the ticket is taken.
+      float* mine = part + ((long)c * nh + h) * PW;
+      __hip_atomic_store(mine + d, o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (d == 0) {
+        __hip_atomic_store(mine + D, mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(mine + D + 1, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+  }
+  if (nsplit == 1) return;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) ticket_s = __hip_atomic_fetch_add(p.tickets + pair, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (ticket_s != (unsigned)(nsplit - 1)) return;
+  for (int i = tid; i < nh * D; i += 64 * WAVES) {
+    const int h = i / D, d = i % D;
+    float gm = -INFINITY, l = 0.f, o = 0.f;
+    for (int s0 = 0; s0 < nsplit; s0 += 8) {               // eight chunks' loads in flight together
+      float pm[8], pl[8], po[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float* ps = part + ((long)min(s0 + u, nsplit - 1) * nh + h) * PW;
+        pm[u] = __hip_atomic_load(ps + D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        pl[u] = __hip_atomic_load(ps + D + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        po[u] = __hip_atomic_load(ps + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (s0 + u < nsplit) {
+          const float nm = fmaxf(gm, pm[u]);
+          const float a = __builtin_amdgcn_exp2f(gm - nm), w = __builtin_amdgcn_exp2f(pm[u] - nm);
+          l = l * a + pl[u] * w;
+          o = o * a + po[u] * w;
+          gm = nm;
+        }
+    }
+    orow[i] = (bf16)(o / l * vscale);
+  }
+  if (tid == 0) __hip_atomic_store(p.tickets + pair, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // ready for the next launch
+}
+
+// What both entry points ask of a cache; 0 when it is sound.
+int check_cache(const bagel_paged_cache* c, const char* who) {
+  BAGEL_CHECK(c && c->k && c->v, "%s: null cache", who);
+  BAGEL_CHECK(c->head_dim == 128 || c->head_dim == 64, "%s: head_dim %d not supported (128 or 64)", who, c->head_dim);
+  BAGEL_CHECK(c->num_kv_heads > 0 && c->num_pages > 0, "%s: %d kv heads, %d pages", who, c->num_kv_heads, c->num_pages);
+  BAGEL_CHECK(c->page_size >= 8 && (c->page_size & (c->page_size - 1)) == 0, "%s: page_size %d is not a power of two of at least 8", who,
+              c->page_size);
+  BAGEL_CHECK((long)c->num_pages * c->page_size <= 0x7fffffffL, "%s: %d pages of %d slots: slots are numbered in 32 bits", who, c->num_pages,
+              c->page_size);
+  BAGEL_CHECK(c->e4m3 == 0 || c->e4m3 == 1, "%s: e4m3=%d", who, c->e4m3);
+  BAGEL_CHECK(!c->e4m3 || (c->k_scale && c->v_scale), "%s: an e4m3 cache needs k_scale and v_scale", who);
+  const long step = c->e4m3 ? 16 : 8;   // elements in 16 bytes
+  BAGEL_CHECK(((uintptr_t)c->k | (uintptr_t)c->v) % 16 == 0 &&
+                  (c->k_page_stride | c->k_slot_stride | c->k_head_stride | c->v_page_stride | c->v_slot_stride | c->v_head_stride) % step == 0,
+              "%s: pages, slots and heads of the cache must start on 16-byte boundaries", who);
+  BAGEL_CHECK(c->k_slot_stride >= c->head_dim && c->v_slot_stride >= c->head_dim && c->k_page_stride >= c->head_dim &&
+                  c->v_page_stride >= c->head_dim && c->k_head_stride >= c->head_dim && c->v_head_stride >= c->head_dim,
+              "%s: a stride of the cache is below head_dim", who);
+  return 0;
+}
+
+Pool pool_of(void* base, long page, long slot, long head, const void* scale, int e4m3) {
+  const long item = e4m3 ? 1 : 2;
+  return Pool{(char*)base, page * item, slot * item, head * item, e4m3 ? (const float*)scale : nullptr};
+}
+Pool k_pool(const bagel_paged_cache* c) { return pool_of(c->k, c->k_page_stride, c->k_slot_stride, c->k_head_stride, c->k_scale, c->e4m3); }
+Pool v_pool(const bagel_paged_cache* c) { return pool_of(c->v, c->v_page_stride, c->v_slot_stride, c->v_head_stride, c->v_scale, c->e4m3); }
+
+// Chunks a row is split into when no row has more than max_kv_len keys.
+int attend_splits(long rows, int Hq, int Hkv, long max_kv_len) {
+  const long pairs = rows * Hkv * ((Hq / Hkv + 15) / 16);
+  const long want = (2L * bagel_cu_count() + pairs - 1) / pairs;     // two workgroups per CU
+  return (int)std::max<long>(1, std::min<long>(std::min<long>(want, MAX_SPLITS), max_kv_len / 256));
+}
+long ticket_bytes(long rows, int Hq, int Hkv) { return (rows * Hkv * ((Hq / Hkv + 15) / 16) * 4 + 255) / 256 * 256; }
+
+}  // namespace
+
+extern "C" int bagel_paged_kv_append_bf16(const void* qkv, long ld, int rows, int Hq, const bagel_paged_cache* cache, const void* q_norm,
+                                          const void* k_norm, const void* cos_table, const void* sin_table, int table_rows,
+                                          const void* row_cs, const void* row_slot, void* Q, long ldq, float eps, int und_rounding,
+                                          void* stream) {
+  if (int rc = check_cache(cache, "bagel_paged_kv_append_bf16")) return rc;
+  const int D = cache->head_dim, Hkv = cache->num_kv_heads;
+  BAGEL_CHECK(rows >= 0 && Hq >= 0, "bagel_paged_kv_append_bf16: rows=%d Hq=%d", rows, Hq);
+  if (rows == 0) return 0;
+  BAGEL_CHECK(qkv && row_slot, "bagel_paged_kv_append_bf16: null operand");
+  BAGEL_CHECK(!cos_table == !sin_table && !cos_table == !row_cs && (!cos_table || table_rows > 0),
+              "bagel_paged_kv_append_bf16: the rotation needs cos_table, sin_table, table_rows and row_cs together");
+  BAGEL_CHECK(ld % 8 == 0 && ld >= (long)(Hq + 2 * Hkv) * D, "bagel_paged_kv_append_bf16: bad leading dim");
+  BAGEL_CHECK(!Q || (ldq % 8 == 0 && ldq >= (long)Hq * D), "bagel_paged_kv_append_bf16: bad leading dim of Q");
+  BAGEL_CHECK(((uintptr_t)qkv | (uintptr_t)Q | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)cos_table | (uintptr_t)sin_table) % 16 == 0,
+              "bagel_paged_kv_append_bf16: misaligned operand");
+  AppendParams p;
+  p.qkv = (const bf16*)qkv; p.ld = ld; p.q_w = (const bf16*)q_norm; p.k_w = (const bf16*)k_norm;
+  p.cos_t = (const bf16*)cos_table; p.sin_t = (const bf16*)sin_table;
+  p.row_cs = (const int*)row_cs; p.row_slot = (const int*)row_slot; p.Q = (bf16*)Q; p.ldq = ldq;
+  p.k = k_pool(cache); p.v = v_pool(cache);
+  p.capacity = (long)cache->num_pages * cache->page_size;
+  p.rows = rows; p.Hq = Hq; p.Hkv = Hkv; p.page_shift = __builtin_ctz(cache->page_size); p.cs_rows = table_rows;
+  p.und_rounding = und_rounding; p.eps = eps;
+  const long threads = (long)rows * (Hq + 2 * Hkv) * (D / 8);
+  BAGEL_CHECK((threads + 255) / 256 <= 0x7fffffffL, "bagel_paged_kv_append_bf16: %d rows are too many for one launch", rows);
+  const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
+  hipStream_t st = (hipStream_t)stream;
+  if (D == 128 && !cache->e4m3) hipLaunchKernelGGL((paged_append_kernel<128, false>), grid, block, 0, st, p);
+  else if (D == 128) hipLaunchKernelGGL((paged_append_kernel<128, true>), grid, block, 0, st, p);
+  else if (!cache->e4m3) hipLaunchKernelGGL((paged_append_kernel<64, false>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((paged_append_kernel<64, true>), grid, block, 0, st, p);
+  BAGEL_LAUNCH_CHECK();
+  return 0;
+}
+
+extern "C" long bagel_paged_decode_attention_workspace_bytes(int rows, int Hq, int Hkv, int head_dim, long max_kv_len) {
+  if (rows <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0 || max_kv_len < 0) return 0;
+  const long splits = attend_splits(rows, Hq, Hkv, max_kv_len);
+  return ticket_bytes(rows, Hq, Hkv) + (splits > 1 ? (long)rows * Hq * splits * (head_dim + 2) * 4 : 0);
+}
+
+extern "C" int bagel_paged_decode_attention_bf16(const void* Q, long ldq, int rows, int Hq, const bagel_paged_cache* cache,
+                                                 const void* page_table, long table_stride, int table_width, const void* kv_lens,
+                                                 long max_kv_len, void* O, long ldo, float softmax_scale, void* workspace,
+                                                 long workspace_bytes, void* stream) {
+  if (int rc = check_cache(cache, "bagel_paged_decode_attention_bf16")) return rc;
+  const int D = cache->head_dim, Hkv = cache->num_kv_heads;
+  BAGEL_CHECK(rows >= 0 && rows <= 65535, "bagel_paged_decode_attention_bf16: rows=%d (at most 65535)", rows);
+  BAGEL_CHECK(Hq > 0 && Hq % Hkv == 0, "bagel_paged_decode_attention_bf16: Hq=%d is not a multiple of the cache's %d kv heads", Hq, Hkv);
+  if (rows == 0) return 0;
+  BAGEL_CHECK(Q && O && page_table && kv_lens && workspace, "bagel_paged_decode_attention_bf16: null operand");
+  BAGEL_CHECK(table_width > 0 && table_stride >= table_width, "bagel_paged_decode_attention_bf16: page table of %d pages, stride %ld",
+              table_width, table_stride);
+  BAGEL_CHECK(ldq % 8 == 0 && ldq >= (long)Hq * D && ldo % 8 == 0 && ldo >= (long)Hq * D,
+              "bagel_paged_decode_attention_bf16: bad leading dim");
+  BAGEL_CHECK(((uintptr_t)Q | (uintptr_t)O | (uintptr_t)workspace) % 16 == 0, "bagel_paged_decode_attention_bf16: misaligned operand");
+  const int blocks = (Hq / Hkv + 15) / 16;
+  BAGEL_CHECK((long)Hkv * blocks <= 65535, "bagel_paged_decode_attention_bf16: too many heads");
+  const long room = (long)table_width * cache->page_size;
+  BAGEL_CHECK(room <= 1L << 30, "bagel_paged_decode_attention_bf16: a page table of %d pages of %d slots (at most 2^30 keys a row)",
+              table_width, cache->page_size);
+  const long bound = max_kv_len > 0 ? std::min(max_kv_len, room) : room;
+  const long need = bagel_paged_decode_attention_workspace_bytes(rows, Hq, Hkv, D, bound);
+  BAGEL_CHECK(workspace_bytes >= need, "bagel_paged_decode_attention_bf16: workspace of %ld bytes, %ld needed", workspace_bytes, need);
+  AttendParams p;
+  p.Q = (const bf16*)Q; p.ldq = ldq; p.k = k_pool(cache); p.v = v_pool(cache);
+  p.table = (const int*)page_table; p.table_stride = table_stride; p.table_width = table_width; p.num_pages = cache->num_pages;
+  p.page_shift = __builtin_ctz(cache->page_size); p.kv_lens = (const int*)kv_lens; p.O = (bf16*)O; p.ldo = ldo;
+  p.tickets = (unsigned*)workspace; p.part = (float*)((char*)workspace + ticket_bytes(rows, Hq, Hkv));
+  p.Hq = Hq; p.Hkv = Hkv;
+  const int splits = attend_splits(rows, Hq, Hkv, bound);
+  p.chunk = (int)((bound + splits - 1) / splits + 127) / 128 * 128;
+  p.scale_log2 = 1.4426950408889634f * (softmax_scale != 0.f ? softmax_scale : 1.0f / sqrtf((float)D));
+  const dim3 grid(splits, Hkv * blocks, rows), block(64 * WAVES);
+  hipStream_t st = (hipStream_t)stream;
+  if (D == 128 && !cache->e4m3) hipLaunchKernelGGL((paged_attention_kernel<128, false>), grid, block, 0, st, p);
+  else if (D == 128) hipLaunchKernelGGL((paged_attention_kernel<128, true>), grid, block, 0, st, p);
+  else if (!cache->e4m3) hipLaunchKernelGGL((paged_attention_kernel<64, false>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((paged_attention_kernel<64, true>), grid, block, 0, st, p);
+  BAGEL_LAUNCH_CHECK();
+  return 0;
+}

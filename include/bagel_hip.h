@@ -222,6 +222,55 @@ int bagel_decode_attention_bf16(const void* qkv, long ld, int rows, int Hq, int 
                                 float eps, int und_rounding, long max_kv_len, void* workspace, long workspace_bytes,
                                 void* stream);
 
+/* ---- a paged key-value cache: requests of any length over one pool of pages -------------------------------------
+ * No counterpart in the reference, whose NaiveCache is re-merged for every token (qwen2_navit.py:574-581); the operators
+ * take the place of the cache append and flash_attn_varlen_func of a decode step (:549-599 driven by
+ * bagel.py:1551-1587) for callers that serve many requests at once.
+ * Element (page, slot, kv head, d) of a pool is at page * page_stride + slot * slot_stride + head * head_stride + d
+ * (elements), so [page][slot][head][D], [page][head][slot][D] and views into a larger array all serve.  page_size: a power of two of
+ * at least 8.  head_dim 128 or 64.  Pages, slots and heads start on 16-byte boundaries.  A slot's number is
+ * page * page_size + (slot in the page), below 2^31.
+ * e4m3 != 0: elements are OCP e4m3 and k_scale / v_scale [num_kv_heads] fp32 hold what one stored unit stands for. */
+typedef struct bagel_paged_cache {
+  void *k, *v;
+  long k_page_stride, k_slot_stride, k_head_stride;
+  long v_page_stride, v_slot_stride, v_head_stride;
+  int num_pages, page_size, num_kv_heads, head_dim, e4m3;
+  const void *k_scale, *v_scale;
+} bagel_paged_cache;
+
+/* Append: q/k RMSNorm + RoPE of every row and its key / value to slot row_slot[row] of the cache, the rotated queries to Q.
+ *   qkv [rows][ld]   Hq query heads, the cache's kv heads of keys, as many of values, each of head_dim (bf16)
+ *   q_norm, k_norm   [head_dim] bf16, each may be NULL: no norm
+ *   cos_table, sin_table [table_rows][head_dim] bf16, row_cs [rows] int32: as in bagel_qk_norm_rope_kv_bf16; all three
+ *                    NULL: no rotation (e.g. to copy keys that are already rotated)
+ *   Q [rows][ldq]    may be NULL (queries not asked for) and may be the query part of qkv
+ * und_rounding as in bagel_qk_norm_rope_kv_bf16; otherwise everything is fp32 up to the one rounding to the stored type
+ * (an e4m3 cache: value / scale clamped to +-448, round to nearest even).
+ * A row with a negative slot is padding: neither the cache nor its Q row is touched.  A row whose slot is not in the
+ * cache or whose row_cs is not in the table stores nothing and its Q row becomes NaN.  The slots of one call must
+ * differ from each other. */
+int bagel_paged_kv_append_bf16(const void* qkv, long ld, int rows, int Hq, const bagel_paged_cache* cache, const void* q_norm,
+                               const void* k_norm, const void* cos_table, const void* sin_table, int table_rows,
+                               const void* row_cs, const void* row_slot, void* Q, long ldq, float eps, int und_rounding,
+                               void* stream);
+
+/* Attention of one new token per row over its first kv_lens[row] keys (its own, appended before, among them):
+ *   O[row][h] = softmax(scale * Q[row][h] . K) V,   any Hq / num_kv_heads
+ *   page_table [rows][table_stride] int32: row's key i is slot i % page_size of page page_table[row][i / page_size];
+ *   entries behind the last key are not read.  kv_lens [rows] int32; 0 or less (a free slot of a batch) gives zeros.
+ * Keys behind kv_lens in the last page may hold anything.  A page id outside the pool, or more keys than table_width
+ * pages hold, makes the outputs of that row (those of the kv heads that met it) NaN; nothing outside the pool is read.
+ * max_kv_len: an upper bound of kv_lens (sizes the split over the length; 0 = unknown, table_width pages; a bound that is too small
+ * costs time, not keys).  softmax_scale 0: 1 / sqrt(head_dim).
+ * workspace: bagel_paged_decode_attention_workspace_bytes() for that bound, zero before the first call (left with zero tickets);
+ * calls that share one must not overlap, be they on two streams or in two replayed graphs.  rows <= 65535. */
+long bagel_paged_decode_attention_workspace_bytes(int rows, int Hq, int Hkv, int head_dim, long max_kv_len);
+int bagel_paged_decode_attention_bf16(const void* Q, long ldq, int rows, int Hq, const bagel_paged_cache* cache,
+                                      const void* page_table, long table_stride, int table_width, const void* kv_lens,
+                                      long max_kv_len, void* O, long ldo, float softmax_scale, void* workspace,
+                                      long workspace_bytes, void* stream);
+
 /* One layer, in place on r->X.  K_ws [Hkv][S][D] and Vt_ws [Hkv][D][S] are THIS layer's workspace slices.
  * next_norm_gen / next_norm_und (optional): weights of the RMSNorm that follows the layer (the next layer's
  * input_layernorm); when given, Xn holds that norm of the layer's output on return. */
