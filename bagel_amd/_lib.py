@@ -20,7 +20,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libbagel_hip.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "bagel_hip.h")
-SOURCES = ["capi.hip", "gemm.hip", "skinny.hip", "attention.hip", "elementwise.hip", "vae.hip", "layer.hip", "decode_attention.hip", "paged.hip"]
+SOURCES = ["capi.hip", "gemm.hip", "skinny.hip", "attention.hip", "elementwise.hip", "vae.hip", "layer.hip", "decode_attention.hip", "paged.hip",
+           "sample.hip"]
 
 # Packed fp32 arithmetic is kept out of the generated code: some forms of v_pk_{add,mul,fma}_f32 are not reliable here,
 # and the compiler makes them from ordinary scalar float code.
@@ -98,7 +99,8 @@ def lib() -> ctypes.CDLL:
         _lib = ctypes.CDLL(variant if variant else LIB_PATH)
         _lib.bagel_last_error.restype = ctypes.c_char_p
         for name in ("bagel_skinny_gemm_workspace_bytes", "bagel_cfg_workspace_bytes", "bagel_groupnorm_workspace_bytes",
-                     "bagel_decode_attention_workspace_bytes", "bagel_paged_decode_attention_workspace_bytes"):
+                     "bagel_decode_attention_workspace_bytes", "bagel_paged_decode_attention_workspace_bytes",
+                     "bagel_sample_rows_workspace_bytes"):
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = ctypes.c_long
     return _lib
@@ -496,6 +498,31 @@ def paged_decode_attention(Q, cache: PagedCache, page_table, kv_lens, O, workspa
               softmax_scale or 0.0, a[4], workspace.numel() * workspace.element_size(), _stream()),
            "bagel_paged_decode_attention_bf16")
     return O
+
+
+# ---- sampling ------------------------------------------------------------------------------------
+def sample_rows_workspace_bytes(rows, n) -> int:
+    return int(lib().bagel_sample_rows_workspace_bytes(I(rows), I(n)))
+
+
+def sample_rows(logits, uniforms, tokens, workspace, temperature=None, top_k=None, top_p=None, min_p=None, logprobs=None):
+    """One token per row of ``logits`` [rows, n] (bfloat16 or float32, rows may be strided) from the caller's ``uniforms``
+    in [0, 1): temperature, then top-k, top-p and min-p (bagel_sample_rows).  The settings are tensors of one value per
+    row, float32 and for top_k int32; None leaves a step out.  ``tokens`` int32, ``logprobs`` float32 (may be None)."""
+    _require(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32) and (logits.stride(1) == 1 or logits.shape[1] == 1),
+             f"sample_rows: bfloat16 or float32 logits [rows, tokens] with contiguous rows expected, got {logits.dtype} {tuple(logits.shape)}")
+    rows, n = logits.shape
+    for name, t, dtype in (("uniforms", uniforms, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("tokens", tokens, torch.int32),
+                           ("logprobs", logprobs, torch.float32)):
+        _require(t is None or (t.dtype == dtype and t.shape == (rows,) and t.is_contiguous()),
+                 f"sample_rows: {name} must be contiguous {dtype} [{rows}]")
+    _require(workspace.is_contiguous(), "sample_rows: contiguous workspace expected")
+    a = _here(logits, uniforms, temperature, top_k, top_p, min_p, tokens, logprobs, workspace)
+    fn = _declared("bagel_sample_rows", VP, L, I, I, I, VP, VP, VP, VP, VP, VP, VP, VP, L, VP)
+    _check(fn(a[0], logits.stride(0) if rows > 1 else n, rows, n, int(logits.dtype == torch.float32), a[1], a[2], a[3], a[4], a[5], a[6],
+              a[7], a[8], workspace.numel() * workspace.element_size(), _stream()), "bagel_sample_rows")
+    return tokens
 
 
 def mot_forward(dims: MotDims, layers, n_layers, rows: MotRows, K_ws, Vt_ws, kv_only_last=False, final_norm_gen=None,

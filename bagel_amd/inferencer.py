@@ -183,14 +183,14 @@ class InterleaveInferencer:
         return Image.fromarray(pixels.to(torch.uint8).cpu().numpy())
 
     @torch.no_grad()
-    def gen_text(self, gen_context, max_length=500, do_sample=True, temperature=1.0, return_tokens=False):
+    def gen_text(self, gen_context, max_length=500, do_sample=True, temperature=1.0, return_tokens=False, **sampling):
         """Decode up to ``max_length`` tokens after the context (which is left untouched) and return the text between
-        the chat markers."""
+        the chat markers.  ``sampling``: generate_text's top_k, top_p, min_p and uniforms."""
         ctx = GenContext.of(gen_context)
         start = self.model.prepare_start_tokens(ctx["kv_lens"], ctx["ropes"], self.new_token_ids)
         tokens = self.model.generate_text(past_key_values=ctx["past_key_values"], max_length=max_length,
                                           do_sample=do_sample, temperature=temperature,
-                                          end_token_id=self.new_token_ids["eos_token_id"], **start)[:, 0]
+                                          end_token_id=self.new_token_ids["eos_token_id"], **sampling, **start)[:, 0]
         text = self.tokenizer.decode(tokens)
         text = text.split("<|im_end|>")[0].split("<|im_start|>")[1]
         return (text, tokens.tolist()) if return_tokens else text

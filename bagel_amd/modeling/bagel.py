@@ -259,11 +259,15 @@ class Bagel:
     @torch.no_grad()
     def generate_text(self, past_key_values: NaiveCache, packed_key_value_indexes, key_values_lens, packed_start_tokens,
                       packed_query_position_ids, max_length: int, do_sample: bool = False, temperature: float = 1.0,
-                      end_token_id: int = None, logits_trace: Optional[list] = None):
+                      end_token_id: int = None, logits_trace: Optional[list] = None, top_k: int = 0, top_p: float = 1.0,
+                      min_p: float = 0.0, uniforms: Optional[torch.Tensor] = None):
         """bagel.py:1526-1596.  Returns the fed tokens ``[steps, B]`` (the start token first).  Greedy decoding
         (``do_sample=False``) is fully on HIP kernels; with ``do_sample=True`` the token is drawn with
         torch.multinomial from softmax(logits / temperature), as the reference does (its draws depend on the
-        device RNG and are not reproducible across implementations either).  The given cache is not modified."""
+        device RNG and are not reproducible across implementations either).  The given cache is not modified.
+        Additions (not in the reference): with ``top_k`` > 0, ``top_p`` < 1, ``min_p`` > 0 or ``uniforms`` the sampled token comes from
+        the sampling kernel (bagel_sample_rows); ``uniforms`` [max_length, B] in [0, 1) fixes the draws, otherwise they
+        are taken from the device RNG."""
         cpu = lambda t: t.detach().cpu()  # noqa: E731
         kvl = [int(x) for x in cpu(key_values_lens).tolist()]
         ki = cpu(packed_key_value_indexes).tolist()
@@ -281,13 +285,42 @@ class Bagel:
                 ctx_v.append(None)
             c += n
         sample_fn = None
-        if do_sample:
+        if not (top_k >= 0 and 0 <= top_p <= 1 and min_p >= 0):
+            raise ValueError(f"top_k={top_k}, top_p={top_p}, min_p={min_p}")
+        if not do_sample and uniforms is not None:
+            raise ValueError("uniforms are given but do_sample is False")
+        if do_sample and (top_k > 0 or top_p < 1 or min_p > 0 or uniforms is not None):
+            sample_fn = self._sampler(len(kvl), max_length, temperature, top_k, top_p, min_p, uniforms)
+        elif do_sample:
             def sample_fn(logits):
                 probs = torch.softmax(logits.float() / temperature, dim=-1)
                 return torch.multinomial(probs, num_samples=1).squeeze(1)
         return self.engine.decode_tokens(cpu(packed_start_tokens).tolist(), cpu(packed_query_position_ids).tolist(), kvl,
                                          ctx_k, ctx_v, max_length, end_token_id=end_token_id, sample_fn=sample_fn,
                                          logits_trace=logits_trace)
+
+    def _sampler(self, B, max_length, temperature, top_k, top_p, min_p, uniforms):
+        """A decode loop's sampling step on the sampling kernel: settings, scratch and random numbers of every step are
+        made once."""
+        dev = self.device
+        if uniforms is None:
+            uniforms = torch.rand((max_length, B), device=dev)
+        elif tuple(uniforms.shape) != (max_length, B):
+            raise ValueError(f"uniforms of shape {tuple(uniforms.shape)}, ({max_length}, {B}) expected")
+        u = uniforms.to(device=dev, dtype=torch.float32).contiguous()
+        n = self.engine.w.lm_head.shape[0]
+        row = lambda v, dtype: torch.full((B,), v, device=dev, dtype=dtype)  # noqa: E731
+        t, p, m = row(temperature, torch.float32), row(top_p, torch.float32), row(min_p, torch.float32)
+        k = row(min(top_k, n), torch.int32)
+        tokens = row(0, torch.int32)
+        ws = torch.empty(K.sample_rows_workspace_bytes(B, n), device=dev, dtype=torch.uint8)
+        step = [0]
+
+        def sample_fn(logits):
+            K.sample_rows(logits, u[step[0]], tokens, ws, temperature=t, top_k=k, top_p=p, min_p=m)
+            step[0] += 1
+            return tokens
+        return sample_fn
 
     def prepare_vae_latent(self, curr_kvlens, curr_rope, image_sizes, new_token_ids):
         """bagel.py:1145-1201."""

@@ -319,6 +319,25 @@ int bagel_taylor_eval_bf16(const void* factors, long factor_stride, int rows, in
 /* out[r] = index of the first maximum of logits[r][0..n) (int32): torch.argmax at bagel.py:1580. */
 int bagel_argmax_rows_bf16(const void* logits, long ld, int rows, int n, void* out_i32, void* stream);
 
+/* Sampling: one token per row of logits [rows][ld] (bf16, or fp32 with logits_f32 != 0; n tokens, at most 2^20) - in
+ * place of softmax + torch.multinomial at bagel.py:1575-1578, with the filters that serving adds and with the random
+ * numbers given.  ld 0: every row draws from the same logits.  temperature, top_p, min_p, uniforms [rows] fp32, top_k [rows] int32; each but uniforms may be NULL.
+ *   w_i = exp((x_i - max) / temperature); tokens in descending order of x, equal ones in ascending order of index
+ *   top_k:  the first k of the order (k <= 0 or >= n: all)
+ *   top_p:  of these the fewest first ones whose weights reach top_p of them all (>= 1: all; always one at least)
+ *   min_p:  of these the ones with w_i >= min_p (<= 0: all; always the first)
+ *   tokens[row] = the first at which the running sum of the weights kept exceeds uniforms[row] x their sum
+ *   logprobs[row] (may be NULL) = ln of its share of the weights kept
+ * Weights are computed in 64 bits and summed exactly in units of 2^-44 (2^-42 at the largest n), so a row's token does
+ * not depend on the launch, the other rows or any order of threads; weights below half a unit are zero.  temperature
+ * <= 0 (or NaN): the first maximum, logprob 0.  NaN logits count as -inf; a row of nothing else gives token 0 with
+ * logprob -inf; +inf logits share all the weight.  uniforms outside [0, 1) act as the nearer end.
+ * workspace: bagel_sample_rows_workspace_bytes(), any content; calls that share one must not overlap.  rows <= 65535. */
+long bagel_sample_rows_workspace_bytes(int rows, int n);
+int bagel_sample_rows(const void* logits, long ld, int rows, int n, int logits_f32, const void* uniforms, const void* temperature,
+                      const void* top_k, const void* top_p, const void* min_p, void* tokens, void* logprobs, void* workspace,
+                      long workspace_bytes, void* stream);
+
 /* CFG combine + renorm + Euler update: bagel.py:1466-1500 and :1339.
  *   renorm_type 0 "global", 1 "channel", 2 "text_channel"; v_* are [rows][P] bf16 (P == 64);
  *   x_t fp32 [rows][P] is updated in place: x_t -= bf16(v_t * dt); x_bf16 receives bf16(x_t);
