@@ -365,9 +365,11 @@ def decode_attention(qkv, Hq, Hkv, D, q_norm, k_norm, cos_t, sin_t, row_cs, row_
 
 
 # ---- a paged key-value cache ---------------------------------------------------------------------
-# The calls of a serving loop are short on the device, so what can be checked once is checked when a PagedCache is made,
-# and the argument types are declared to ctypes instead of being wrapped per call.
+# A step of a serving loop is a few microseconds on the device, so these wrappers are written for the host's time too: what
+# can be checked once is checked when a PagedCache is made, argument types are declared to ctypes instead of being wrapped
+# per call, messages are only made when something is wrong (an append: 5 us on the host; 17 us without all this).
 E4M3 = torch.float8_e4m3fn
+BF16 = torch.bfloat16
 
 
 def _require(ok, message):
@@ -375,30 +377,26 @@ def _require(ok, message):
         raise RuntimeError(message)
 
 
-def _here(*tensors):
-    """Addresses of tensors (None: 0) that must live on the current device."""
+def _not_here(*tensors):
+    """Raises for the first tensor that does not live on the current device."""
     for t in tensors:
-        _require(t is None or t.is_cuda, "device tensor expected")
-    dev = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
+        if t is not None:
+            _require(t.is_cuda, "device tensor expected")
             _p(t)      # raises, and names both devices
-    return [0 if t is None else t.data_ptr() for t in tensors]
 
 
-def _rows(t, width, name):
-    """Row stride of a [rows, ...] bf16 tensor whose rows are ``width`` contiguous elements."""
+def _check_rows(t, width, name):
+    """A bf16 tensor whose rows are ``width`` contiguous elements, by its stride where it is not contiguous as a whole."""
     n = 1
     for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
         _require(size == 1 or stride == n, f"{name}: the elements of a row must be contiguous")
         n *= size
-    _require(t.dtype == torch.bfloat16 and n == width, f"{name}: {t.dtype} rows of {n} elements, bfloat16 rows of {width} expected")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    _require(t.dtype == BF16 and n == width, f"{name}: {t.dtype} rows of {n} elements, bfloat16 rows of {width} expected")
+    return t.stride(0) if t.shape[0] > 1 else width
 
 
-def _ints(t, shape, name):
-    _require(t.dtype == torch.int32 and t.shape == shape and t.is_contiguous(),
-             f"{name}: contiguous int32 {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}")
+def _wrong_values(t, dtype, shape, name):
+    raise RuntimeError(f"{name} must be contiguous {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
 
 
 class _PagedCacheStruct(ctypes.Structure):
@@ -428,6 +426,7 @@ class PagedCache:
         self.k_pages, self.v_pages, self.k_scale, self.v_scale = k_pages, v_pages, k_scale, v_scale
         held = [t for t in (k_pages, v_pages, k_scale, v_scale) if t is not None]
         _require(all(t.device == k_pages.device for t in held), "paged cache: pools and scales on different devices")
+        self.device_index = k_pages.get_device()      # -1 on the host: refused by the calls, not here
         addr = [0 if t is None else t.data_ptr() for t in (k_pages, v_pages, k_scale, v_scale)]
         # a dimension of one element has no stride of its own
         strides = [t.stride(d) if t.shape[d] > 1 else self.head_dim for t in (k_pages, v_pages) for d in range(3)]
@@ -436,38 +435,76 @@ class PagedCache:
         self.ref = ctypes.byref(self.struct)
 
 
+_functions = {}
+
+
 def _declared(name, *types):
-    fn = getattr(lib(), name)
-    if fn.argtypes is None:
+    """The entry point with its argument types declared; types are only looked at the first time."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
         fn.argtypes = types
+        _functions[name] = fn
     return fn
+
+
+def _raw_stream(dev):
+    """The current stream of device ``dev`` (checked to be the current one) as an address."""
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def paged_kv_append(qkv, Hq, cache: PagedCache, row_slot, Q=None, q_norm=None, k_norm=None, cos_t=None, sin_t=None, row_cs=None,
                     eps=1e-6, und_rounding=False):
     """q/k norm + RoPE of qkv's rows; keys and values to the cache's slots ``row_slot`` (negative: padding, left alone), the
     queries to ``Q`` [rows, Hq, head_dim] (bagel_paged_kv_append_bf16).  No norm weight: no norm; no tables: no rotation."""
-    rows, D = qkv.shape[0], cache.head_dim
-    _require(Hq >= 0 and (Hq > 0 or Q is None), "paged_kv_append: Q without query heads")
-    ld = _rows(qkv, (Hq + 2 * cache.heads) * D, "paged_kv_append: qkv")
-    _ints(row_slot, (rows,), "paged_kv_append: row_slot")
-    ldq = 0
+    rows, D = len(qkv), cache.head_dim
+    if Hq < 0 or (Hq == 0 and Q is not None):
+        raise RuntimeError(f"paged_kv_append: Q without query heads (Hq={Hq})")
+    width = (Hq + 2 * cache.heads) * D
+    if qkv.dtype is BF16 and qkv.dim() == 2 and qkv.size(1) == width and qkv.is_contiguous():
+        ld = width
+    else:
+        ld = _check_rows(qkv, width, "paged_kv_append: qkv")
+    dev = torch.cuda.current_device() if qkv.is_cuda else -2
+    here = qkv.get_device() == dev == cache.device_index == row_slot.get_device()
+    if row_slot.dtype is not torch.int32 or row_slot.dim() != 1 or len(row_slot) != rows or not row_slot.is_contiguous():
+        _wrong_values(row_slot, torch.int32, (rows,), "paged_kv_append: row_slot")
+    q_addr = ldq = 0
     if Q is not None:
-        _require(Q.shape[0] == rows, f"paged_kv_append: Q has {Q.shape[0]} rows, qkv {rows}")
-        ldq = _rows(Q, Hq * D, "paged_kv_append: Q")
-    for w in (q_norm, k_norm):
-        _require(w is None or (w.dtype == torch.bfloat16 and w.shape == (D,) and w.is_contiguous()),
-                 f"paged_kv_append: norm weights are contiguous bfloat16 [{D}]")
-    _require((cos_t is None) == (sin_t is None) == (row_cs is None), "paged_kv_append: cos_t, sin_t and row_cs come together")
-    if cos_t is not None:
-        _require(cos_t.dtype == sin_t.dtype == torch.bfloat16 and cos_t.dim() == 2 and cos_t.shape[1] == D and
-                 cos_t.shape == sin_t.shape and cos_t.is_contiguous() and sin_t.is_contiguous(),
-                 f"paged_kv_append: rotation tables are contiguous bfloat16 [positions, {D}]")
-        _ints(row_cs, (rows,), "paged_kv_append: row_cs")
-    a = _here(qkv, row_slot, Q, q_norm, k_norm, cos_t, sin_t, row_cs, cache.k_pages)
+        if len(Q) != rows:
+            raise RuntimeError(f"paged_kv_append: Q has {len(Q)} rows, qkv {rows}")
+        if Q.dtype is BF16 and Q.dim() == 3 and Q.size(1) == Hq and Q.size(2) == D and Q.is_contiguous():
+            ldq = Hq * D
+        else:
+            ldq = _check_rows(Q, Hq * D, "paged_kv_append: Q")
+        here = here and Q.get_device() == dev
+        q_addr = Q.data_ptr()
+    norms = [0, 0]
+    for i, w in enumerate((q_norm, k_norm)):
+        if w is not None:
+            if w.dtype is not BF16 or w.dim() != 1 or len(w) != D or not w.is_contiguous():
+                _wrong_values(w, BF16, (D,), "paged_kv_append: norm weights")
+            here = here and w.get_device() == dev
+            norms[i] = w.data_ptr()
+    cos_addr = sin_addr = cs_addr = table_rows = 0
+    if cos_t is not None and sin_t is not None and row_cs is not None:
+        table_rows = len(cos_t)
+        for t in (cos_t, sin_t):
+            if t.dtype is not BF16 or t.dim() != 2 or t.size(1) != D or len(t) != table_rows or not t.is_contiguous():
+                _wrong_values(t, BF16, (table_rows, D), "paged_kv_append: rotation tables")
+        if row_cs.dtype is not torch.int32 or row_cs.dim() != 1 or len(row_cs) != rows or not row_cs.is_contiguous():
+            _wrong_values(row_cs, torch.int32, (rows,), "paged_kv_append: row_cs")
+        here = here and cos_t.get_device() == sin_t.get_device() == row_cs.get_device() == dev
+        cos_addr, sin_addr, cs_addr = cos_t.data_ptr(), sin_t.data_ptr(), row_cs.data_ptr()
+    elif not (cos_t is None and sin_t is None and row_cs is None):
+        raise RuntimeError("paged_kv_append: cos_t, sin_t and row_cs come together")
+    if not here:
+        _not_here(qkv, row_slot, Q, q_norm, k_norm, cos_t, sin_t, row_cs, cache.k_pages)
     fn = _declared("bagel_paged_kv_append_bf16", VP, L, I, I, VP, VP, VP, VP, VP, I, VP, VP, VP, L, F, I, VP)
-    _check(fn(a[0], ld, rows, Hq, cache.ref, a[3], a[4], a[5], a[6], 0 if cos_t is None else cos_t.shape[0], a[7], a[1], a[2], ldq,
-              eps, 1 if und_rounding else 0, _stream()), "bagel_paged_kv_append_bf16")
+    rc = fn(qkv.data_ptr(), ld, rows, Hq, cache.ref, norms[0], norms[1], cos_addr, sin_addr, table_rows, cs_addr, row_slot.data_ptr(), q_addr,
+            ldq, eps, 1 if und_rounding else 0, _raw_stream(dev))
+    if rc:
+        _check(rc, "bagel_paged_kv_append_bf16")
     return Q
 
 
@@ -480,23 +517,34 @@ def paged_decode_attention(Q, cache: PagedCache, page_table, kv_lens, O, workspa
     Q, O [rows, Hq, head_dim]; page_table [rows, pages] int32; workspace: paged_decode_attention_workspace_bytes, made with
     torch.zeros; max_kv_len: an upper bound of kv_lens known on the host (0: the table's width)."""
     D = cache.head_dim
-    _require(Q.dim() == 3 and Q.shape == O.shape and Q.shape[2] == D and Q.shape[1] > 0 and Q.shape[1] % cache.heads == 0,
-             f"paged_decode_attention: Q {tuple(Q.shape)} and O {tuple(O.shape)} must be [rows, a multiple of {cache.heads} heads, {D}]")
-    rows, Hq = Q.shape[0], Q.shape[1]
-    ldq, ldo = _rows(Q, Hq * D, "paged_decode_attention: Q"), _rows(O, Hq * D, "paged_decode_attention: O")
-    _require(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == rows and page_table.shape[1] > 0 and
-             page_table.stride(1) == 1, f"paged_decode_attention: page_table must be int32 [{rows}, pages] with contiguous rows")
-    _ints(kv_lens, (rows,), "paged_decode_attention: kv_lens")
-    _require(max_kv_len >= 0, "paged_decode_attention: max_kv_len is negative")
-    _require(softmax_scale is None or (softmax_scale != 0 and math.isfinite(softmax_scale)),
-             f"paged_decode_attention: softmax_scale {softmax_scale}")
-    _require(workspace.is_contiguous(), "paged_decode_attention: contiguous workspace expected")
-    a = _here(Q, page_table, kv_lens, O, workspace, cache.k_pages)
-    width = page_table.shape[1]
+    if Q.dim() != 3 or Q.shape != O.shape or Q.size(2) != D or Q.size(1) == 0 or Q.size(1) % cache.heads:
+        raise RuntimeError(f"paged_decode_attention: Q {tuple(Q.shape)} and O {tuple(O.shape)} must be [rows, a multiple of "
+                           f"{cache.heads} heads, {D}]")
+    rows, Hq = len(Q), Q.size(1)
+    ldq = Hq * D if Q.dtype is BF16 and Q.is_contiguous() else _check_rows(Q, Hq * D, "paged_decode_attention: Q")
+    ldo = Hq * D if O.dtype is BF16 and O.is_contiguous() else _check_rows(O, Hq * D, "paged_decode_attention: O")
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or len(page_table) != rows or page_table.size(1) == 0 or \
+            page_table.stride(1) != 1:
+        raise RuntimeError(f"paged_decode_attention: page_table must be int32 [{rows}, pages] with contiguous rows, got "
+                           f"{page_table.dtype} {list(page_table.shape)}")
+    if kv_lens.dtype is not torch.int32 or kv_lens.dim() != 1 or len(kv_lens) != rows or not kv_lens.is_contiguous():
+        _wrong_values(kv_lens, torch.int32, (rows,), "paged_decode_attention: kv_lens")
+    if max_kv_len < 0:
+        raise RuntimeError(f"paged_decode_attention: max_kv_len {max_kv_len}")
+    if softmax_scale is not None and (softmax_scale == 0 or not math.isfinite(softmax_scale)):
+        raise RuntimeError(f"paged_decode_attention: softmax_scale {softmax_scale}")
+    if not workspace.is_contiguous():
+        raise RuntimeError("paged_decode_attention: contiguous workspace expected")
+    dev = torch.cuda.current_device() if Q.is_cuda else -2
+    if not (Q.get_device() == dev == O.get_device() == page_table.get_device() == kv_lens.get_device() == workspace.get_device() ==
+            cache.device_index):
+        _not_here(Q, page_table, kv_lens, O, workspace, cache.k_pages)
+    width = page_table.size(1)
     fn = _declared("bagel_paged_decode_attention_bf16", VP, L, I, I, VP, VP, L, I, VP, L, VP, L, F, VP, L, VP)
-    _check(fn(a[0], ldq, rows, Hq, cache.ref, a[1], page_table.stride(0) if rows > 1 else width, width, a[2], max_kv_len, a[3], ldo,
-              softmax_scale or 0.0, a[4], workspace.numel() * workspace.element_size(), _stream()),
-           "bagel_paged_decode_attention_bf16")
+    rc = fn(Q.data_ptr(), ldq, rows, Hq, cache.ref, page_table.data_ptr(), page_table.stride(0) if rows > 1 else width, width,
+            kv_lens.data_ptr(), max_kv_len, O.data_ptr(), ldo, softmax_scale or 0.0, workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
+    if rc:
+        _check(rc, "bagel_paged_decode_attention_bf16")
     return O
 
 
@@ -509,19 +557,32 @@ def sample_rows(logits, uniforms, tokens, workspace, temperature=None, top_k=Non
     """One token per row of ``logits`` [rows, n] (bfloat16 or float32, rows may be strided) from the caller's ``uniforms``
     in [0, 1): temperature, then top-k, top-p and min-p (bagel_sample_rows).  The settings are tensors of one value per
     row, float32 and for top_k int32; None leaves a step out.  ``tokens`` int32, ``logprobs`` float32 (may be None)."""
-    _require(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32) and (logits.stride(1) == 1 or logits.shape[1] == 1),
-             f"sample_rows: bfloat16 or float32 logits [rows, tokens] with contiguous rows expected, got {logits.dtype} {tuple(logits.shape)}")
+    if logits.dim() != 2 or logits.dtype not in (BF16, torch.float32) or (logits.stride(1) != 1 and logits.size(1) != 1):
+        raise RuntimeError(f"sample_rows: bfloat16 or float32 logits [rows, tokens] with contiguous rows expected, got {logits.dtype} "
+                           f"{tuple(logits.shape)}")
     rows, n = logits.shape
+    dev = torch.cuda.current_device() if logits.is_cuda else -2
+    here = logits.get_device() == dev == workspace.get_device()
+    addr = []
     for name, t, dtype in (("uniforms", uniforms, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
                            ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("tokens", tokens, torch.int32),
                            ("logprobs", logprobs, torch.float32)):
-        _require(t is None or (t.dtype == dtype and t.shape == (rows,) and t.is_contiguous()),
-                 f"sample_rows: {name} must be contiguous {dtype} [{rows}]")
-    _require(workspace.is_contiguous(), "sample_rows: contiguous workspace expected")
-    a = _here(logits, uniforms, temperature, top_k, top_p, min_p, tokens, logprobs, workspace)
+        if t is None:
+            addr.append(0)
+            continue
+        if t.dtype is not dtype or t.dim() != 1 or len(t) != rows or not t.is_contiguous():
+            _wrong_values(t, dtype, (rows,), "sample_rows: " + name)
+        here = here and t.get_device() == dev
+        addr.append(t.data_ptr())
+    if not workspace.is_contiguous():
+        raise RuntimeError("sample_rows: contiguous workspace expected")
+    if not here:
+        _not_here(logits, uniforms, temperature, top_k, top_p, min_p, tokens, logprobs, workspace)
     fn = _declared("bagel_sample_rows", VP, L, I, I, I, VP, VP, VP, VP, VP, VP, VP, VP, L, VP)
-    _check(fn(a[0], logits.stride(0) if rows > 1 else n, rows, n, int(logits.dtype == torch.float32), a[1], a[2], a[3], a[4], a[5], a[6],
-              a[7], a[8], workspace.numel() * workspace.element_size(), _stream()), "bagel_sample_rows")
+    rc = fn(logits.data_ptr(), logits.stride(0) if rows > 1 else n, rows, n, 1 if logits.dtype is torch.float32 else 0, *addr,
+            workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
+    if rc:
+        _check(rc, "bagel_sample_rows")
     return tokens
 
 
