@@ -4,48 +4,72 @@
 // filter keeps a prefix of that order: top-k its first k, top-p the shortest prefix whose weights reach p of the weights
 // that top-k left, min-p the tokens with w_i >= m.  The token drawn is the first whose running sum of weights exceeds
 // u x (the kept weights).  A border of one of these sums decides a whole token, so sums have to be better than fp32 and
-// must not depend on the order in which threads come by: a weight is computed in 64 bits and then counted in whole units
-// of 2^-44 (2^-43, 2^-42 beyond 2^18, 2^19 tokens, so that a row's sum stays below 2^63); integer sums are exact in any
-// order, atomics included.  A token below half a unit (31 T under the maximum) has no weight.
+// must not depend on the order in which threads come by.
 //
-// No row is sorted.  One histogram over the value - 2048 bins of equal width from the maximum down to where weights
-// vanish, each with its count and its weight - finds the bin that holds a border; only that bin's tokens are gathered
-// and sorted, by (value, index) as one 64-bit key.  A bin of too many tokens (equal or nearly equal logits) is first narrowed by histograms
-// over that key's bits, eleven at a time, which ends at a single token at the latest.
+// No row is sorted.  Tokens are counted into bins of 1/32 octave of weight: with v = 32 log2(e) x / T, token x is in bin
+// floor(v), and weighs 2^(frac(v) / 32), between 1 and 1.022, in that bin's unit, which is computed in 64 bits (to 2^-33) and
+// counted as an integer in steps of 2^-32.  Integer sums are exact in any order, LDS atomics included, and bins and weights
+// depend neither on the maximum nor on how a row is cut up: so the logits are read ONCE, in slices that know nothing of
+// each other, and each slice's histogram reaches 44 octaves below its own maximum (what lies below weighs less than 2^-44 of
+// the first token: nothing).  Where bins are added up, a bin's sum is brought to steps of 2^-42 of the first bin's unit.
+//
+// Two launches.  The first: a workgroup per slice, whose logits stay in registers: maximum, histogram, and a list of the
+// slice's foremost tokens as (value, index) keys of 64 bits.  Bound by its instructions and LDS atomics, some twenty and one a
+// logit: a bin's count and weight are the two parts of one 64-bit word.  The second: one workgroup per row, in one of three ways:
+//   - a top-k of a few: the lists hold it, whatever the row's weights are, so the first launch only counted tokens (without weights),
+//     and the listed tokens are sorted;
+//   - a top-p whose border lies among the listed tokens: they are sorted, and everything else is prefix sums over them;
+//   - else each border is resolved by itself: its bin comes from the histogram, and the tokens of that bin alone, gathered from the
+//     lists or, further down, from the row, are sorted.  A bin of too many tokens (equal or nearly equal logits) is first
+//     narrowed by histograms over the key's bits, eleven at a time, which ends at a single token at the latest.
+// Up to 64 tokens are sorted and summed by one wave in its registers.
 #include "common.h"
 #include <algorithm>
+#include <type_traits>
 #include "../../include/bagel_hip.h"
 
 namespace {
 
 typedef unsigned long long u64;
 
-constexpr int BINS = 2048;
+constexpr int OCTAVE = 32;           // bins per octave of weight
+constexpr int BINS = 44 * OCTAVE;
+constexpr int STEPS_LOG2 = 32;       // 2^32 steps to a bin's unit: 2^20 tokens of one bin stay below 2^53
+constexpr int FINER = 10;            // bins are added up in steps of 2^-(32 + 10) of the first bin's unit
+constexpr int COUNT_SHIFT = 48;      // a slice's bin: steps (2^15 tokens stay below 2^48), and the count above them
+constexpr int SUB = 2048;            // bins of a narrowing histogram
 constexpr int CAP = 4096;            // tokens that are sorted at once
-constexpr int MAX_SLICES = 32;       // workgroups per row
+constexpr int LIST = 1024;           // tokens that a slice lists at most
+constexpr int FEW = 1024;            // a top-k up to here is looked for in the lists first
 constexpr int THREADS = 1024;
-constexpr float WINDOW = 31.25f;     // exp(-31.25) < 2^-45: half a unit
+constexpr int CHUNK = 8 * THREADS;   // logits that a workgroup loads at a time
+constexpr int MAX_SLICES = 128;      // 2^20 logits in single chunks
+
+struct Slice {       // what the first launch says of a slice
+  u64 best;          // the order key of its first maximum (where it is not greedy: of the maximum and no index)
+  int listed, cut;   // tokens in its list; the last of its bins (from its own first) that the list holds
+};
 
 struct Params {
   const void* logits;
   long ld;
-  int n, slices, shift;              // shift: a unit of weight is 2^-shift
+  int n, slices;
   bool vec;                          // rows start on 16-byte boundaries
   const float *uniforms, *temperature, *top_p, *min_p;
   const int* top_k;
   int* tokens;
   float* logprobs;
-  u64* best;                         // [rows][MAX_SLICES] smallest order key of each slice
-  u64* mass;                         // [rows][BINS]
-  unsigned* count;                   // [rows][BINS]
+  Slice* slice;                      // [rows][slices]
+  u64* list;                         // [rows][slices][LIST], in no order
+  u64* bins;                         // [rows][slices][BINS] count << COUNT_SHIFT | steps
 };
 
-// A NaN counts as a masked token; the two zeros are one value.
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
+// A NaN counts as a masked token: the maximum of a NaN and a number is the number.
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }
 
-// Ascending in the order of the tokens: descending value, then ascending index.
+// Ascending in the order of the tokens: descending value (the two zeros are one), then ascending index.
 __device__ __forceinline__ u64 order_key(float x, int i) {
-  const unsigned b = __float_as_uint(x);
+  const unsigned b = __float_as_uint(x + 0.0f);
   const unsigned up = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
   return ((u64)~up << 32) | (unsigned)i;
 }
@@ -54,157 +78,200 @@ __device__ __forceinline__ float key_value(u64 key) {
   return __uint_as_float(up ^ ((up >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-struct Scale {       // of one row
-  float top, per;    // maximum; bins per unit of value
-  double inv_t;
-  double unit;       // 2^shift
+// Bins counted down from that of a maximum `top`.
+struct Scale {
+  float top;
+  double per;        // 32 log2(e) / T
+  double base;       // bin of the maximum
 };
-__device__ __forceinline__ Scale make_scale(float top, float t, int shift) {
-  return Scale{top, (BINS - 1) / WINDOW / t, 1.0 / (double)t, __builtin_ldexp(1.0, shift)};
-}
-
-// Monotone in x; the last bin is that of the tokens without weight.
-__device__ __forceinline__ int bin_of(float x, const Scale& s) {
+constexpr double LN2 = 0.69314718055994530942;
+__device__ __forceinline__ Scale make_scale(float top, float t) {
 #pragma clang fp contract(off)
-  const float v = (s.top - x) * s.per;
-  return x == s.top ? 0 : v < (float)(BINS - 1) ? (int)v : BINS - 1;
+  const double per = OCTAVE / LN2 / (double)t;
+  return Scale{top, per, __builtin_floor((double)top * per)};
 }
-
-constexpr double LN2_HIGH = 2977044471.0 / 4294967296.0;   // floor(2^32 ln 2) / 2^32
-constexpr double LN2_LOW = 1.90821492927058770002e-10;    // the rest of ln 2
-
-// exp(z) for z <= 0 in 64 bits: 2^n exp(r), |r| <= ln 2 / 2, the exponential series to r^13 (its next term is below 2^-57).
-__device__ __forceinline__ double exp64(double z) {
-  const double n = __builtin_rint(z * 1.4426950408889634074);
-  double r = __builtin_fma(n, -LN2_HIGH, z);          // exact: n and the 32 bits of the first part leave room
-  r = __builtin_fma(n, -LN2_LOW, r);
-  double p = 1.0 / 6227020800.0;
-  p = __builtin_fma(p, r, 1.0 / 479001600.0);
-  p = __builtin_fma(p, r, 1.0 / 39916800.0);
-  p = __builtin_fma(p, r, 1.0 / 3628800.0);
-  p = __builtin_fma(p, r, 1.0 / 362880.0);
-  p = __builtin_fma(p, r, 1.0 / 40320.0);
-  p = __builtin_fma(p, r, 1.0 / 5040.0);
-  p = __builtin_fma(p, r, 1.0 / 720.0);
-  p = __builtin_fma(p, r, 1.0 / 120.0);
-  p = __builtin_fma(p, r, 1.0 / 24.0);
-  p = __builtin_fma(p, r, 1.0 / 6.0);
-  p = __builtin_fma(p, r, 0.5);
-  p = __builtin_fma(p, r, 1.0);
-  p = __builtin_fma(p, r, 1.0);
-  return __builtin_ldexp(p, (int)n);
-}
-__device__ __forceinline__ double weight(float x, const Scale& s) {   // of a token that is not in the last bin
+// Token x's bin, BINS for one that weighs nothing, and `part` = v - floor(v).  The maximum is in bin 0 even where v is no
+// number (an infinite maximum, an infinite T).
+__device__ __forceinline__ int bin_of(float x, const Scale& s, double& part) {
 #pragma clang fp contract(off)
-  return x == s.top ? 1.0 : exp64(((double)x - (double)s.top) * s.inv_t);
-}
-// The weight in units, rounded to nearest: a sum with 2^52 leaves it in the low bits.
-__device__ __forceinline__ u64 units(double w, const Scale& s) {
-  return (u64)__double_as_longlong(__builtin_fma(w, s.unit, 4503599627370496.0)) & ((1ull << 52) - 1);
-}
-
-// f(value, index) for this thread's share of tokens [from, to) of a row; from is a multiple of 8.
-template <typename T, typename F>
-__device__ __forceinline__ void for_each(const Params& p, int row, int from, int to, F f) {
-  const T* x = (const T*)p.logits + (long)row * p.ld;
-  for (int i = from + 8 * (int)threadIdx.x; i < to; i += 8 * THREADS) {
-    float v[8];
-    if (p.vec && i + 8 <= to) {
-      if constexpr (sizeof(T) == 2) {
-        const bf16x8 w = *(const bf16x8*)(x + i);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (float)w[e];
-      } else {
-        const f32x4 a = *(const f32x4*)(x + i), b = *(const f32x4*)(x + i + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = a[e];
-          v[4 + e] = b[e];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = i + e < to ? (float)x[i + e] : 0.f;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (i + e < to) f(clean(v[e]), i + e);
+  const double v = (double)x * s.per, d = s.base - __builtin_floor(v);
+  part = __builtin_amdgcn_fract(v);
+  if (x == s.top) {
+    part = part == part ? part : 0.0;
+    return 0;
   }
+  return d < (double)BINS ? (int)d : BINS;
+}
+__device__ __forceinline__ int bin_of(float x, const Scale& s) {
+  double part;
+  return bin_of(x, s, part);
+}
+// The next value, up or down, in the order of the values.
+__device__ __forceinline__ float next(float x, int step) {
+  const unsigned u = __float_as_uint(x), up = (u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u)) + step;
+  return __uint_as_float(up ^ ((up >> 31) ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ float before(float x) { return next(x, -1); }
+// The smallest value in a bin up to `b`: x is in one of them just when it is not below.
+__device__ __forceinline__ float edge_of(int b, const Scale& s) {
+#pragma clang fp contract(off)
+  if (s.top == INFINITY) return s.top;
+  const double lowest = s.base - b;
+  auto inside = [&](float x) { return (double)x * s.per >= lowest; };
+  if (!(s.per > 0.0)) return -3.402823466e38f;      // an infinite T: every value is in the maximum's bin
+  float x = (float)(lowest / s.per);                // off by a step or two
+  for (int i = 0; i < 4 && x > -INFINITY && inside(x); ++i) x = next(x, -1);
+  for (int i = 0; i < 8 && x < s.top && !inside(x); ++i) x = next(x, 1);
+  return x;
+}
+// 2^(part / 32) in steps: a cubic through its values at the four Chebyshev points of [0, 1] (7e-11 of it off at most); a sum
+// with 2^52 leaves the rounded steps in the low bits.
+struct Cubic {
+  double c3 = 1.71230584268166556e-06 * (1ull << STEPS_LOG2), c2 = 2.34584642666360913e-04 * (1ull << STEPS_LOG2);
+  double c1 = 2.16608517052938078e-02 * (1ull << STEPS_LOG2), c0 = 9.99999999927715377e-01 * (1ull << STEPS_LOG2) + 4503599627370496.0;
+  // kept in scalar registers: otherwise every use first copies them to vector registers
+  __device__ __forceinline__ void settle() { asm volatile("" : "+s"(c3), "+s"(c2), "+s"(c1), "+s"(c0)); }
+  __device__ __forceinline__ u64 steps(double part) const {
+    double p = __builtin_fma(part, c3, c2);
+    p = __builtin_fma(p, part, c1);
+    p = __builtin_fma(p, part, c0);
+    return (u64)__double_as_longlong(p) & ((1ull << 52) - 1);
+  }
+};
+__device__ __forceinline__ u64 steps_of(double part) { return Cubic().steps(part); }
+// Steps of bin b in the finer ones of bin 0; table: 2^(-j / 32).  Exact for b = 0: equal logits share out exactly.
+__device__ __forceinline__ u64 scaled(u64 steps, int b, const double* table) {
+  return (u64)__builtin_rint(__builtin_ldexp((double)steps * table[b % OCTAVE], FINER - b / OCTAVE));
+}
+// 2^(-j / 32) for j = 0 ... 31, by the exponential series.
+struct Table {
+  double at[OCTAVE];
+  constexpr Table() : at() {
+    for (int j = 0; j < OCTAVE; ++j) {
+      double term = 1.0, sum = 1.0;
+      for (int i = 1; i < 24; ++i) sum += term *= -LN2 * j / OCTAVE / i;
+      at[j] = sum;
+    }
+  }
+};
+__constant__ const Table powers;
+
+// The whole part of f x whole, 0 <= f <= 1, or with `up` the next whole number at or above it: exact, since tokens of
+// equal weight put sums precisely on these borders.
+__device__ __forceinline__ u64 part_of(float f, u64 whole, bool up) {
+  if (!(f > 0.f)) return 0;
+  int e;
+  const u64 m = (u64)(frexpf(f, &e) * 16777216.f);       // f = m 2^(e - 24)
+  const int sh = 24 - e;                                  // 23 for f = 1, up to 172
+  const u64 low = m * whole, high = __umul64hi(m, whole);
+  u64 part, rest;
+  if (sh < 64) {
+    part = (high << (64 - sh)) | (low >> sh);
+    rest = low & ((1ull << sh) - 1);
+  } else if (sh < 128) {
+    part = sh == 64 ? high : high >> (sh - 64);
+    rest = low | (sh == 64 ? 0 : high & ((1ull << (sh - 64)) - 1));
+  } else {
+    part = 0;
+    rest = 1;
+  }
+  return part + (up && rest ? 1 : 0);
 }
 
 __device__ __forceinline__ u64 shfl_u64(u64 v, int from) {
   return ((u64)(unsigned)__shfl((int)(v >> 32), from) << 32) | (unsigned)__shfl((int)(unsigned)v, from);
 }
-
-// ---- first launch: the maximum of every slice (as the order key, so the first maximum), and an empty histogram
-template <typename T>
-__global__ __launch_bounds__(THREADS) void sample_top_kernel(Params p) {
-  const int row = blockIdx.y, slice = blockIdx.x;
-  const int per = ((p.n + p.slices - 1) / p.slices + 7) / 8 * 8;
-  const int from = min(slice * per, p.n), to = min(from + per, p.n);
-  for (int b = slice * THREADS + threadIdx.x; b < BINS; b += p.slices * THREADS) {
-    p.mass[(long)row * BINS + b] = 0;
-    p.count[(long)row * BINS + b] = 0;
-  }
-  u64 best = ~0ull;
-  for_each<T>(p, row, from, to, [&](float x, int i) { best = min(best, order_key(x, i)); });
+// The smallest key of all lanes, in all of them.
+__device__ __forceinline__ u64 wave_min(u64 v) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) best = min(best, shfl_u64(best, (threadIdx.x & 63) ^ o));
-  __shared__ u64 s[THREADS / 64];
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = best;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < THREADS / 64; ++w) best = min(best, s[w]);
-    p.best[(long)row * MAX_SLICES + slice] = best;
+  for (int o = 32; o > 0; o >>= 1) v = min(v, shfl_u64(v, (threadIdx.x & 63) ^ o));
+  return v;
+}
+
+// The value of lane ^ W.
+template <int W>
+__device__ __forceinline__ unsigned xor_u32(unsigned v) {
+  typedef __attribute__((ext_vector_type(2))) unsigned u32x2_;
+  if constexpr (W < 16) return __float_as_uint(xor_lane<W>(__uint_as_float(v)));
+  const u32x2_ a = W == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return threadIdx.x & W ? a[0] : a[1];
+}
+// One key per lane -> ascending over the wave: a bitonic network in registers.
+template <int Q, int J>
+__device__ __forceinline__ void wave_sort_step(u64& key) {
+  const u64 other = ((u64)xor_u32<J>((unsigned)(key >> 32)) << 32) | xor_u32<J>((unsigned)key);
+  const bool up = (threadIdx.x & Q) == 0 || Q == 64, lower = (threadIdx.x & J) == 0;
+  key = (up == lower) == (other < key) ? other : key;
+  if constexpr (J > 1) wave_sort_step<Q, J / 2>(key);
+}
+__device__ __forceinline__ void wave_sort(u64& key) {
+  wave_sort_step<2, 1>(key);
+  wave_sort_step<4, 2>(key);
+  wave_sort_step<8, 4>(key);
+  wave_sort_step<16, 8>(key);
+  wave_sort_step<32, 16>(key);
+  wave_sort_step<64, 32>(key);
+}
+
+// Eight logits from index i on (a multiple of 8), -inf behind the row's end.
+template <typename T>
+__device__ __forceinline__ void load8(const Params& p, const T* row, int i, float (&v)[8]) {
+  if (p.vec && i + 8 <= p.n) {
+    if constexpr (sizeof(T) == 2) {
+      const bf16x8 w = *(const bf16x8*)(row + i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = clean((float)w[e]);
+    } else {
+      const f32x4 a = *(const f32x4*)(row + i), b = *(const f32x4*)(row + i + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = clean(a[e]);
+        v[4 + e] = clean(b[e]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = i + e < p.n ? clean((float)row[i + e]) : -INFINITY;
+  }
+}
+// f(value, index) for this thread's share of a whole row, four loads in flight.
+template <typename T, typename F>
+__device__ __forceinline__ void for_each(const Params& p, int row, F f) {
+  const T* x = (const T*)p.logits + (long)row * p.ld;
+  for (int i0 = 0; i0 < p.n; i0 += 4 * CHUNK) {
+    float v[4][8];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) load8(p, x, i0 + c * CHUNK + 8 * (int)threadIdx.x, v[c]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f(v[c][e], i0 + c * CHUNK + 8 * (int)threadIdx.x + e);
   }
 }
 
-__device__ __forceinline__ u64 row_best(const Params& p, int row) {
-  u64 best = ~0ull;
-  for (int s = 0; s < p.slices; ++s) best = min(best, p.best[(long)row * MAX_SLICES + s]);
-  return best;
-}
-__device__ __forceinline__ float row_temperature(const Params& p, int row) { return p.temperature ? p.temperature[row] : 1.0f; }
-
-// ---- second launch: counts and weights of the bins
-template <typename T>
-__global__ __launch_bounds__(THREADS) void sample_histogram_kernel(Params p) {
-  const int row = blockIdx.y, slice = blockIdx.x;
-  const float t = row_temperature(p, row), top = key_value(row_best(p, row));
-  if (!(t > 0.f) || top == -INFINITY) return;       // greedy, or nothing to choose from
-  const Scale s = make_scale(top, t, p.shift);
-  __shared__ u64 mass[BINS];
-  __shared__ unsigned count[BINS];
-  for (int b = threadIdx.x; b < BINS; b += THREADS) mass[b] = 0, count[b] = 0;
-  __syncthreads();
-  const int per = ((p.n + p.slices - 1) / p.slices + 7) / 8 * 8;
-  const int from = min(slice * per, p.n), to = min(from + per, p.n);
-  for_each<T>(p, row, from, to, [&](float x, int i) {
-    const int b = bin_of(x, s);
-    if (b < BINS - 1) {                              // those of the last bin are what is left
-      atomicAdd(&count[b], 1u);
-      atomicAdd(&mass[b], units(weight(x, s), s));
-    }
-  });
-  __syncthreads();
-  for (int b = threadIdx.x; b < BINS; b += THREADS)
-    if (count[b]) {
-      atomicAdd(p.count + (long)row * BINS + b, count[b]);
-      atomicAdd(p.mass + (long)row * BINS + b, mass[b]);
-    }
-}
-
-// ---- third launch: one workgroup per row finds the borders and the token
 struct Sums {
   u64 mass;
   unsigned count;
 };
-struct Hit {         // a token of the order, with the sums up to and including it
-  u64 key;
-  Sums sums;
-};
-
-// Inclusive scan over the workgroup's threads.
+// Inclusive scans over the workgroup's threads.
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const u64 m = shfl_u64(v, max(lane - o, 0));
+    if (lane >= o) v += m;
+  }
+  return v;
+}
+__device__ __forceinline__ u64 scan(u64 v, u64* per_wave, int stride) {
+  const int wave = threadIdx.x >> 6;
+  v = wave_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) per_wave[wave * stride] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) v += per_wave[w * stride];
+  return v;
+}
 __device__ __forceinline__ Sums scan(Sums v, Sums* per_wave) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -225,12 +292,219 @@ __device__ __forceinline__ Sums scan(Sums v, Sums* per_wave) {
   }
   return v;
 }
+// Bins -> sums up to and including them (two neighbours per thread).
+template <int N>
+__device__ __forceinline__ void prefix(u64* packed, Sums* per_wave) {
+  static_assert(N <= 2 * THREADS && N % 2 == 0, "two bins per thread");
+  const int t = threadIdx.x;
+  u64 a = 0, b = 0;
+  __syncthreads();
+  if (2 * t < N) a = packed[2 * t], b = packed[2 * t + 1];
+  const u64 v = scan(a + b, &per_wave->mass, sizeof(Sums) / 8);
+  if (2 * t < N) packed[2 * t] = v - b, packed[2 * t + 1] = v;
+  __syncthreads();
+}
+template <int N>
+__device__ __forceinline__ void prefix(u64* mass, unsigned* count, Sums* per_wave) {
+  static_assert(N <= 2 * THREADS && N % 2 == 0, "two bins per thread");
+  const int t = threadIdx.x;
+  Sums a{0, 0}, b{0, 0};
+  __syncthreads();
+  if (2 * t < N) a = Sums{mass[2 * t], count[2 * t]}, b = Sums{mass[2 * t + 1], count[2 * t + 1]};
+  const Sums v = scan(Sums{a.mass + b.mass, a.count + b.count}, per_wave);
+  if (2 * t < N) {
+    mass[2 * t] = v.mass - b.mass, count[2 * t] = v.count - b.count;
+    mass[2 * t + 1] = v.mass, count[2 * t + 1] = v.count;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ float row_temperature(const Params& p, int row) { return p.temperature ? p.temperature[row] : 1.0f; }
+// A row's top-k: 0 where it leaves nothing out.
+__device__ __forceinline__ int row_top_k(const Params& p, int row) {
+  const int k = p.top_k ? p.top_k[row] : 0;
+  return k >= 1 && k < p.n ? k : 0;
+}
+
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4_;
+// Logits of a chunk as they are loaded.  settle(): what was made of them so far is not kept in registers.
+template <typename T>
+struct Raw;
+template <>
+struct Raw<bf16> {
+  u32x4_ w;
+  __device__ __forceinline__ float raw(int e) const { return __uint_as_float(e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16); }
+  __device__ __forceinline__ float at(int e) const { return clean(raw(e)); }
+  __device__ __forceinline__ void settle() { asm volatile("" : "+v"(w)); }
+};
+template <>
+struct Raw<float> {
+  f32x4 w[2];
+  __device__ __forceinline__ float raw(int e) const { return w[e / 4][e % 4]; }
+  __device__ __forceinline__ float at(int e) const { return clean(raw(e)); }
+  __device__ __forceinline__ void settle() { asm volatile("" : "+v"(w[0]), "+v"(w[1])); }
+};
+
+// ---- first launch: a workgroup per slice of C chunks
+template <typename T, int C>
+__global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
+  const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
+  __shared__ u64 bins[BINS];
+  __shared__ Sums per_wave[THREADS / 64];
+  __shared__ float top_s[THREADS / 64];
+  __shared__ int first, reach, fits;
+  __shared__ unsigned listed;
+  const T* x = (const T*)p.logits + (long)row * p.ld;
+  const int from = slice * C * CHUNK + 8 * tid;
+  Raw<T> v[C];
+  if (p.vec && (slice + 1) * C * CHUNK <= p.n) {       // every load at once
+#pragma unroll
+    for (int c = 0; c < C; ++c) v[c] = *(const Raw<T>*)(x + from + c * CHUNK);
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      T w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = from + c * CHUNK + e < p.n ? x[from + c * CHUNK + e] : (T)-INFINITY;
+      v[c] = __builtin_bit_cast(Raw<T>, w);
+    }
+  }
+  const float t = row_temperature(p, row);
+  const int k = row_top_k(p, row);
+  const bool few = k >= 1 && k <= FEW;
+  for (int b = tid; b < BINS; b += THREADS) bins[b] = 0;
+  if (tid == 0) first = 0x7fffffff, reach = BINS - 1, fits = -1, listed = 0;
+  float top = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, v[c].at(e));
+  top = wave_max(top);
+  if ((tid & 63) == 0) top_s[wave] = top;
+  __syncthreads();
+  static_assert(THREADS / 64 == 16, "a lane per wave");
+  top = row_reduce(top_s[tid & 15], [](float a, float b) { return fmaxf(a, b); });
+  auto settle = [&] {
+#pragma unroll
+    for (int c = 0; c < C; ++c) v[c].settle();
+  };
+  settle();
+  Slice* out = p.slice + (long)row * p.slices + slice;
+  if (!(t > 0.f) || top == -INFINITY) {       // greedy, or nothing to choose from here: the first maximum
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int c = C - 1; c >= 0; --c)
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if (v[c].at(e) == top) at = from + c * CHUNK + e;
+    if (at != 0x7fffffff) atomicMin(&first, at);
+    __syncthreads();
+    if (tid == 0) *out = Slice{order_key(top, first), 0, BINS - 1};
+    return;
+  }
+  const Scale s = make_scale(top, t);
+  constexpr u64 ONE = 1ull << COUNT_SHIFT;
+  static_assert(C * CHUNK <= 1 << 15, "a slice's sums fit their half of the word");
+  const float low = before(edge_of(BINS - 1, s));
+  if (s.base > -1e9 && s.base < 1e9 && low > -INFINITY) {
+    // all but the strangest rows: bins as 32-bit integers, and `low`, which is just below the last bin, in place of all values
+    // further down, masked ones and NaN among them: nothing here is infinite
+    const int base = (int)s.base;
+    Cubic cubic;
+    cubic.settle();
+    auto tally = [&](auto weights) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const double y = (double)fmaxf(v[c].raw(e), low) * s.per;
+          const int b = base - (int)__builtin_floor(y);
+          if (b < BINS) {
+            if constexpr (weights.value) atomicAdd(&bins[b], ONE + cubic.steps(__builtin_amdgcn_fract(y)));
+            else atomicAdd(&bins[b], ONE);
+          }
+        }
+    };
+    if (few) tally(std::false_type{});
+    else tally(std::true_type{});
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        double part;
+        const int b = bin_of(v[c].at(e), s, part);
+        if (b < BINS) atomicAdd(&bins[b], ONE + steps_of(part));
+      }
+  }
+  __syncthreads();
+  if (!few) {
+    u64* at = p.bins + ((long)row * p.slices + slice) * BINS;
+    for (int b = tid; b < BINS; b += THREADS) at[b] = bins[b];
+  }
+  // the list: the bins up to `cut`, the last that fits or, for a top-k of a few, the first that brings k tokens
+  prefix<BINS>(bins, per_wave);
+  for (int b = 2 * tid; b < 2 * tid + 2; ++b)
+    if (b < BINS) {
+      const unsigned upto = bins[b] >> COUNT_SHIFT, ahead = b ? bins[b - 1] >> COUNT_SHIFT : 0, after = b < BINS - 1 ? bins[b + 1] >> COUNT_SHIFT : LIST + 1;
+      if (upto <= LIST && after > LIST) fits = b;
+      if (few && upto >= (unsigned)k && ahead < (unsigned)k) reach = b;
+    }
+  __syncthreads();
+  const int cut = min(fits, reach);
+  if (cut >= 0) {
+    u64* list = p.list + ((long)row * p.slices + slice) * LIST;
+    const float edge = edge_of(cut, s);
+    settle();
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v[c].at(e) >= edge) {
+          const unsigned at = atomicAdd(&listed, 1u);
+          if (at < LIST) list[at] = order_key(v[c].at(e), from + c * CHUNK + e);
+        }
+    __syncthreads();
+  }
+  if (tid == 0) *out = Slice{order_key(top, 0), (int)min(listed, (unsigned)LIST), cut};
+}
+
+// ---- second launch: one workgroup per row finds the token
+struct Hit {         // a token of the order, with the steps of bin 0 up to and including it
+  u64 key, mass;
+};
 
 template <typename T>
 __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
   const int row = blockIdx.x, tid = threadIdx.x;
-  const u64 best = row_best(p, row);
-  const float t = row_temperature(p, row), top = key_value(best);
+  __shared__ u64 mass[BINS];                 // steps of bin 0 up to and including a bin
+  __shared__ unsigned count[BINS];
+  __shared__ u64 work[CAP];                  // the tokens being sorted, or the histogram of a narrowing step
+  const double* table = powers.at;
+  __shared__ Sums per_wave[THREADS / 64];
+  __shared__ int first[MAX_SLICES + 1];      // where each slice's list begins when they are put together
+  __shared__ int down[MAX_SLICES];           // a slice's first bin, counted from the row's
+  __shared__ int found, lowest_cut, enough;
+  __shared__ unsigned gathered;
+  __shared__ u64 best_s, edge_s;
+  __shared__ Hit hit_s;
+  u64* sub_mass = work;                      // [SUB]
+  unsigned* sub_count = (unsigned*)(work + SUB);
+
+  Slice mine{~0ull, 0, BINS - 1};
+  if (tid < p.slices) mine = p.slice[(long)row * p.slices + tid];
+  const float t = row_temperature(p, row), top_p = p.top_p ? p.top_p[row] : 1.0f, min_p = p.min_p ? p.min_p[row] : 0.f, u = p.uniforms[row];
+  const int k = row_top_k(p, row);
+  const bool few = k >= 1 && k <= FEW;
+  if (tid == 0) best_s = ~0ull, lowest_cut = BINS, enough = 1, gathered = 0;
+  __syncthreads();
+  if (tid < MAX_SLICES) {
+    const u64 m = wave_min(mine.best);
+    if ((tid & 63) == 0) atomicMin(&best_s, m);
+  }
+  __syncthreads();
+  const u64 best = best_s;
+  const float top = key_value(best);
   if (!(t > 0.f) || top == -INFINITY) {
     if (tid == 0) {
       p.tokens[row] = top == -INFINITY ? 0 : (int)(unsigned)best;
@@ -238,120 +512,296 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
     }
     return;
   }
-  const Scale s = make_scale(top, t, p.shift);
-  __shared__ u64 mass[BINS];                 // sums up to and including a bin
-  __shared__ unsigned count[BINS];
-  __shared__ u64 work[CAP];                  // the tokens being sorted, or the histogram of a narrowing step
-  __shared__ Sums per_wave[THREADS / 64];
-  __shared__ int found;
-  __shared__ unsigned listed;
-  __shared__ Hit hit_s;
-  u64* sub_mass = work;                      // [BINS]
-  unsigned* sub_count = (unsigned*)(work + BINS);
-
-  // two neighbouring bins per thread
-  auto prefix = [&](u64* m, unsigned* c) {
-    __syncthreads();
-    const Sums a{m[2 * tid], c[2 * tid]}, b{m[2 * tid + 1], c[2 * tid + 1]};
-    const Sums v = scan(Sums{a.mass + b.mass, a.count + b.count}, per_wave);
-    m[2 * tid] = v.mass - b.mass, c[2 * tid] = v.count - b.count;
-    m[2 * tid + 1] = v.mass, c[2 * tid + 1] = v.count;
-    __syncthreads();
+  const Scale s = make_scale(top, t);
+  auto place = [&](u64 key, double& part) { return bin_of(key_value(key), s, part); };
+  auto weight = [&](float x) { return x == top ? 1.0 : exp(((double)x - (double)top) / (double)t); };
+  // a token's steps, in those of bin 0
+  auto steps = [&](u64 key) {
+    double part;
+    const int b = place(key, part);
+    return b < BINS ? scaled(steps_of(part), b, table) : 0ull;
   };
-  if (tid == 0) hit_s = Hit{best, Sums{(u64)s.unit, 1}};
-  for (int b = tid; b < BINS; b += THREADS) mass[b] = p.mass[(long)row * BINS + b], count[b] = p.count[(long)row * BINS + b];
-  prefix(mass, count);
-  const u64 total = mass[BINS - 1];
+  const u64 top_steps = steps(best);
+  if (tid == 0) hit_s = Hit{best, top_steps};
+  if (tid < MAX_SLICES) {
+    const float their = key_value(mine.best);
+    const double d = s.base - make_scale(their, t).base;
+    const int off = tid >= p.slices || their == -INFINITY ? BINS : their == top ? 0 : d < (double)BINS ? (int)d : BINS;
+    down[tid] = off;
+    if (off < BINS && mine.cut < BINS - 1) atomicMin(&lowest_cut, mine.cut + off);
+    if (mine.listed < k && mine.cut < BINS - 1) enough = 0;       // tokens of the top k may be missing
+    // this slice's place in the lists put together: a scan over two waves
+    int n = mine.listed;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int m = __shfl_up(n, o);
+      if ((tid & 63) >= o) n += m;
+    }
+    first[tid + 1] = n;
+  }
+  static_assert(MAX_SLICES == 128, "two waves");
+  if (tid == 0) first[0] = 0;
+  __syncthreads();
+  const int half = first[64];
+  __syncthreads();
+  if (tid >= 64 && tid < MAX_SLICES) first[tid + 1] += half;
+  __syncthreads();
+  const int listed = first[MAX_SLICES];
 
-  // the first bin whose sum, on top of `base`, reaches the target; BINS where none does
-  auto find_bin = [&](const u64* m, const unsigned* c, const Sums base, bool by_count, u64 target) {
-    if (tid == 0) found = BINS;
-    __syncthreads();
-    for (int b = 2 * tid; b < 2 * tid + 2; ++b) {
-      const u64 upto = by_count ? (u64)base.count + c[b] : base.mass + m[b];
-      const u64 before = b == 0 ? (by_count ? (u64)base.count : base.mass) : by_count ? (u64)base.count + c[b - 1] : base.mass + m[b - 1];
-      if (before < target && upto >= target) found = b;
+  // f(key) of every listed token, four loads in flight
+  auto for_listed = [&](auto f) {
+    for (int i0 = tid; i0 < listed; i0 += 4 * THREADS) {
+      u64 key[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int i = i0 + c * THREADS;
+        int low = 0, high = p.slices;                  // the last slice that begins at or before i
+        while (high - low > 1) {
+          const int mid = (low + high) / 2;
+          if (first[mid] <= i) low = mid;
+          else high = mid;
+        }
+        key[c] = i < listed ? p.list[((long)row * p.slices + low) * LIST + i - first[low]] : 0;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (i0 + c * THREADS < listed) f(key[c]);
     }
-    __syncthreads();
-    const int b = found;
-    __syncthreads();
-    return b;
   };
-  // the first token of the order at which the count / the weights reach the target, somewhere in `bin`
-  auto resolve = [&](int bin, bool by_count, u64 target) {
-    Sums base{bin ? mass[bin - 1] : 0, bin ? count[bin - 1] : 0};
-    unsigned inside = count[bin] - base.count;
-    u64 low = 0, high = ~0ull;
-    for (int sh = 53; inside > CAP; sh = max(sh - 11, 0)) {
-      __syncthreads();
-      for (int b = tid; b < BINS; b += THREADS) sub_mass[b] = 0, sub_count[b] = 0;
-      __syncthreads();
-      for_each<T>(p, row, 0, p.n, [&](float x, int i) {
-        if (bin_of(x, s) != bin) return;
-        const u64 key = order_key(x, i);
-        if (key < low || key > high) return;
-        const int b = (int)((key - low) >> sh);
-        atomicAdd(&sub_count[b], 1u);
-        atomicAdd(&sub_mass[b], units(weight(x, s), s));
-      });
-      prefix(sub_mass, sub_count);
-      const int b = min(find_bin(sub_mass, sub_count, base, by_count, target), BINS - 1);
-      const Sums before{b ? sub_mass[b - 1] : 0, b ? sub_count[b - 1] : 0};
-      inside = sub_count[b] - before.count;
-      base.mass += before.mass;
-      base.count += before.count;
-      low += (u64)b << sh;
-      high = low + ((1ull << sh) - 1);
-      __syncthreads();
-    }
-    __syncthreads();
-    if (tid == 0) listed = 0;
-    __syncthreads();
-    for_each<T>(p, row, 0, p.n, [&](float x, int i) {
-      if (bin_of(x, s) != bin) return;
-      const u64 key = order_key(x, i);
-      if (key < low || key > high) return;
-      const unsigned at = atomicAdd(&listed, 1u);
-      if (at < CAP) work[at] = key;
-    });
-    __syncthreads();
-    const int len = (int)min(listed, (unsigned)CAP);
+  auto put = [&](u64 key) {
+    const unsigned at = atomicAdd(&gathered, 1u);
+    if (at < CAP) work[at] = key;
+  };
+  auto sort = [&](int len) {
     int size = 2;
     while (size < len) size *= 2;
+    __syncthreads();
     for (int i = len + tid; i < size; i += THREADS) work[i] = ~0ull;
-    for (int k = 2; k <= size; k *= 2)
-      for (int j = k / 2; j > 0; j /= 2) {
+    for (int q = 2; q <= size; q *= 2)
+      for (int j = q / 2; j > 0; j /= 2) {
         __syncthreads();
         for (int i = tid; i < size; i += THREADS) {
           const int o = i ^ j;
           if (o > i) {
             const u64 a = work[i], b = work[o];
-            if ((a > b) == ((i & k) == 0)) work[i] = b, work[o] = a;
+            if ((a > b) == ((i & q) == 0)) work[i] = b, work[o] = a;
           }
         }
       }
     __syncthreads();
-    // four neighbours per thread
-    Sums each[CAP / THREADS], sum{0, 0};
+  };
+  constexpr int EACH = CAP / THREADS;        // neighbours per thread in the sorted order
+  // f(key) of the sorted tokens as sums up to and including each of the thread's own, and up to the one before them
+  auto sums_of = [&](int len, u64& before, u64 (&upto)[EACH], auto f) {
+    u64 sum = 0;
 #pragma unroll
-    for (int e = 0; e < CAP / THREADS; ++e) {
-      const int i = tid * (CAP / THREADS) + e;
-      if (i < len) {
-        sum.mass += units(weight(key_value(work[i]), s), s);
-        sum.count += 1;
-      }
-      each[e] = sum;
+    for (int e = 0; e < EACH; ++e) {
+      const int i = tid * EACH + e;
+      if (i < len) sum += f(work[i]);
+      upto[e] = sum;
     }
-    const Sums all = scan(sum, per_wave);
-    base.mass += all.mass - sum.mass;
-    base.count += all.count - sum.count;
+    before = scan(sum, &per_wave->mass, sizeof(Sums) / 8) - sum;
 #pragma unroll
-    for (int e = 0; e < CAP / THREADS; ++e) {
-      const int i = tid * (CAP / THREADS) + e;
-      const Sums upto{base.mass + each[e].mass, base.count + each[e].count};
-      const Sums before{e ? base.mass + each[e ? e - 1 : 0].mass : base.mass, e ? base.count + each[e ? e - 1 : 0].count : base.count};
-      if (i < len && (by_count ? (before.count < target && upto.count >= target) : (before.mass < target && upto.mass >= target)))
-        hit_s = Hit{work[i], upto};
+    for (int e = 0; e < EACH; ++e) upto[e] += before;
+  };
+  auto answer = [&](u64 key, u64 kept) {               // by one thread
+    p.tokens[row] = (int)(unsigned)key;
+    if (p.logprobs) {
+      const float x = key_value(key);
+      p.logprobs[row] = (float)((x == top ? 0.0 : ((double)x - (double)top) / (double)t) - log((double)kept / (double)top_steps));
+    }
+  };
+  auto p_target = [&](u64 whole) { return max((u64)1, part_of(top_p, whole, true)); };
+  auto u_target = [&](u64 kept) { return 1 + min(part_of(u < 1.0f ? u : u >= 1.0f ? 1.0f : 0.f, kept, false), kept - 1); };
+
+  // the token, from `len` tokens in work that hold everything the filters keep; whole: the weights that top_p is a share of
+  // (of the first k of these where there is a top-k)
+  auto finish = [&](int len, u64 whole) {
+    if (len <= 64) {
+      if (tid >= 64) return;
+      u64 key = tid < len ? work[tid] : ~0ull;
+      wave_sort(key);
+      const u64 sum = wave_scan(tid < len ? steps(key) : 0);
+      // the place at which the sums reach the target (the last one where roundings leave them short)
+      auto place_at = [&](u64 target) {
+        const u64 m = __ballot(tid < len && sum >= target);
+        return m ? __ffsll(m) - 1 : len - 1;
+      };
+      u64 kept = whole;
+      if (k) whole = kept = shfl_u64(sum, min(k, len) - 1);
+      if (top_p < 1.0f) kept = shfl_u64(sum, place_at(p_target(whole)));
+      if (min_p > 0.f) {
+        const u64 m = __ballot(tid < len && sum <= kept && (tid == 0 || weight(key_value(key)) >= (double)min_p));
+        kept = shfl_u64(sum, 63 - __clzll(m));
+      }
+      const int at = place_at(u_target(kept));
+      if (tid == at) answer(key, kept);
+      return;
+    }
+    sort(len);
+    u64 before, upto[EACH];
+    sums_of(len, before, upto, steps);
+    // the token for which `is` holds, given its place in the order and the sums before and up to it
+    auto token_where = [&](auto is) {
+#pragma unroll
+      for (int e = 0; e < EACH; ++e)
+        if (tid * EACH + e < len && is(tid * EACH + e, e ? upto[e ? e - 1 : 0] : before, upto[e])) hit_s = Hit{work[tid * EACH + e], upto[e]};
+      __syncthreads();
+      const Hit h = hit_s;
+      __syncthreads();
+      return h;
+    };
+    // (the last token is taken where the roundings of single tokens and of whole bins leave the sum short)
+    auto token_at = [&](u64 target) {
+      return token_where([&](int i, u64 from, u64 to) { return from < target && (to >= target || i == len - 1); });
+    };
+    u64 kept = whole;
+    if (k) whole = kept = token_where([&](int i, u64, u64) { return i == min(k, len) - 1; }).mass;
+    if (top_p < 1.0f) kept = token_at(p_target(whole)).mass;
+    if (min_p > 0.f) {
+      // a prefix: the largest sum among those that stay
+      if (tid == 0) edge_s = 0;
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int i = tid * EACH + e;
+        if (i < len && upto[e] <= kept && (i == 0 || weight(key_value(work[i])) >= (double)min_p)) atomicMax(&edge_s, upto[e]);
+      }
+      __syncthreads();
+      kept = edge_s;
+    }
+    const Hit h = token_at(u_target(kept));
+    if (tid == 0) answer(h.key, kept);
+  };
+
+  // the bin of N for which `is` holds, given the bin; N where there is none
+  auto find = [&](int n, auto is) {
+    if (tid == 0) found = n;
+    __syncthreads();
+    for (int b = 2 * tid; b < min(2 * tid + 2, n); ++b)
+      if (is(b)) found = b;
+    __syncthreads();
+    const int b = found;
+    __syncthreads();
+    return b;
+  };
+  if (few && enough && listed <= CAP) {
+    float edge = -INFINITY;
+    if (listed > 64) {
+      // of the slices' first k only those in the bins of the row's first k
+      for (int b = tid; b < BINS; b += THREADS) mass[b] = 0;
+      __syncthreads();
+      for_listed([&](u64 key) {
+        const int b = bin_of(key_value(key), s);
+        if (b < BINS) atomicAdd(&mass[b], 1ull);
+      });
+      prefix<BINS>(mass, per_wave);
+      const int b = find(BINS, [&](int b) { return (b == 0 || mass[b - 1] < (u64)k) && mass[b] >= (u64)k; });
+      if (b < BINS) edge = edge_of(b, s);
+    }
+    for_listed([&](u64 key) {
+      if (key_value(key) >= edge) put(key);
+    });
+    __syncthreads();
+    finish((int)min(gathered, (unsigned)CAP), 0);
+    return;
+  }
+
+  // the row's histogram: the slices' or, where the lists of a top-k did not do and weights were left out, made here
+  if (few) {
+    for (int b = tid; b < BINS; b += THREADS) mass[b] = 0, count[b] = 0;
+    __syncthreads();
+    for_each<T>(p, row, [&](float x, int) {
+      double part;
+      const int b = bin_of(x, s, part);
+      if (b < BINS) {
+        atomicAdd(&count[b], 1u);
+        atomicAdd(&mass[b], steps_of(part));
+      }
+    });
+    __syncthreads();
+    for (int b = tid; b < BINS; b += THREADS) mass[b] = scaled(mass[b], b, table);
+  } else {
+    for (int b = tid; b < BINS; b += THREADS) {
+      u64 m = 0;
+      unsigned c = 0;
+#pragma unroll 4
+      for (int i = 0; i < p.slices; ++i) {
+        const int theirs = b - down[i];
+        const u64 both = theirs >= 0 ? p.bins[((long)row * p.slices + i) * BINS + theirs] : 0;
+        m += both & ((1ull << COUNT_SHIFT) - 1);
+        c += (unsigned)(both >> COUNT_SHIFT);
+      }
+      mass[b] = scaled(m, b, table);
+      count[b] = c;
+    }
+  }
+  prefix<BINS>(mass, count, per_wave);
+  const u64 total = mass[BINS - 1];
+
+  auto bin_by_count = [&](u64 target) { return find(BINS, [&](int b) { return (b == 0 || count[b - 1] < target) && count[b] >= target; }); };
+  auto bin_by_mass = [&](u64 target) { return find(BINS, [&](int b) { return (b == 0 || mass[b - 1] < target) && mass[b] >= target; }); };
+
+  // the first token of the order at which the count / the steps reach the target, somewhere in `bin`
+  auto resolve = [&](int bin, bool by_count, u64 target) {
+    const Sums base{bin ? mass[bin - 1] : 0, bin ? count[bin - 1] : 0};      // before the bin
+    Sums inner{0, 0};                                                        // in the bin before what is left of it, in its own steps
+    unsigned inside = count[bin] - base.count;
+    u64 low = 0, high = ~0ull;
+    auto reached = [&](u64 m, unsigned c) {
+      return by_count ? (u64)(base.count + inner.count + c) >= target : base.mass + scaled(inner.mass + m, bin, table) >= target;
+    };
+    const float least = edge_of(bin, s), beyond = bin ? edge_of(bin - 1, s) : INFINITY;
+    auto in_bin = [&](float x, int i, u64& key) {
+      if (!(x >= least && (x < beyond || bin == 0))) return false;
+      key = order_key(x, i);
+      return key >= low && key <= high;
+    };
+    auto part_steps = [&](u64 key) {
+      double part;
+      place(key, part);
+      return steps_of(part);
+    };
+    for (int sh = 53; inside > CAP; sh = max(sh - 11, 0)) {
+      __syncthreads();
+      for (int b = tid; b < SUB; b += THREADS) sub_mass[b] = 0, sub_count[b] = 0;
+      __syncthreads();
+      for_each<T>(p, row, [&](float x, int i) {
+        u64 key;
+        if (!in_bin(x, i, key)) return;
+        const int b = (int)((key - low) >> sh);
+        atomicAdd(&sub_count[b], 1u);
+        atomicAdd(&sub_mass[b], part_steps(key));
+      });
+      prefix<SUB>(sub_mass, sub_count, per_wave);
+      const int b = min(find(SUB, [&](int b) { return (b == 0 || !reached(sub_mass[b - 1], sub_count[b - 1])) && reached(sub_mass[b], sub_count[b]); }), SUB - 1);
+      const Sums before{b ? sub_mass[b - 1] : 0, b ? sub_count[b - 1] : 0};
+      inside = sub_count[b] - before.count;
+      inner.mass += before.mass;
+      inner.count += before.count;
+      low += (u64)b << sh;
+      high = low + ((1ull << sh) - 1);
+      __syncthreads();
+    }
+    __syncthreads();
+    if (tid == 0) gathered = 0;
+    __syncthreads();
+    auto gather = [&](float x, int i) {
+      u64 key;
+      if (in_bin(x, i, key)) put(key);
+    };
+    if (bin <= lowest_cut) for_listed([&](u64 key) { gather(key_value(key), (int)(unsigned)key); });
+    else for_each<T>(p, row, gather);
+    __syncthreads();
+    const int len = (int)min(gathered, (unsigned)CAP);
+    sort(len);
+    u64 before, upto[EACH];
+    sums_of(len, before, upto, part_steps);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int i = tid * EACH + e;
+      if (i < len && (i == 0 || !reached(e ? upto[e ? e - 1 : 0] : before, (unsigned)i)) && (i == len - 1 || reached(upto[e], (unsigned)i + 1)))
+        hit_s = Hit{work[i], base.mass + scaled(inner.mass + upto[e], bin, table)};
     }
     __syncthreads();
     const Hit h = hit_s;
@@ -359,66 +809,75 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
     return h;
   };
 
-  Hit border{~0ull, Sums{total, (unsigned)p.n}};      // the last token kept
-  const int k = p.top_k ? p.top_k[row] : 0;
-  if (k >= 1 && k < p.n) {
-    const int bin = find_bin(mass, count, Sums{0, 0}, true, (u64)k);
-    if (bin < BINS - 1) border = resolve(bin, true, (u64)k);      // further down there is no weight to cut off
+  const int k_bin = k ? bin_by_count((u64)k) : BINS;
+  const bool has_k = k_bin < BINS;                     // further down there is no weight to cut off
+  // everything that stays lies in the bins up to this one
+  const int last_bin = has_k ? k_bin : top_p < 1.0f ? bin_by_mass(p_target(total)) : BINS;
+  if (last_bin <= lowest_cut && last_bin < BINS && count[last_bin] <= CAP && (has_k || !k)) {
+    const float edge = edge_of(last_bin, s);
+    for_listed([&](u64 key) {
+      if (key_value(key) >= edge) put(key);
+    });
+    __syncthreads();
+    finish((int)min(gathered, (unsigned)CAP), total);
+    return;
   }
-  const float top_p = p.top_p ? p.top_p[row] : 1.0f;
+
+  Hit border{~0ull, total};                            // the last token kept
+  if (has_k) border = resolve(k_bin, true, (u64)k);
   if (top_p < 1.0f) {
-    const u64 target = max((u64)1, (u64)__builtin_ceil((double)max(top_p, 0.f) * (double)border.sums.mass));
-    const int bin = find_bin(mass, count, Sums{0, 0}, false, target);
-    if (bin < BINS - 1) border = resolve(bin, false, target);
+    const u64 target = p_target(border.mass);
+    const int bin = bin_by_mass(target);
+    if (bin < BINS) border = resolve(bin, false, target);
   }
-  u64 kept = border.sums.mass;
-  const float min_p = p.min_p ? p.min_p[row] : 0.f;
+  u64 kept = border.mass;
   if (min_p > 0.f) {
-    // the bins that the threshold may lie in, one to each side for the roundings of the bins' borders
-    const double edge = -log((double)min_p) * ((BINS - 1) / (double)WINDOW);
-    const int b0 = edge < 1.0 ? 0 : edge < BINS ? (int)edge - 1 : BINS, b1 = b0 + 3;
-    if (b0 < BINS - 1 && (border.key == ~0ull || bin_of(key_value(border.key), s) >= b0)) {
-      u64 mine = 0;
-      for_each<T>(p, row, 0, p.n, [&](float x, int i) {
-        const int b = bin_of(x, s);
-        if (b < b0 || b > b1 || b >= BINS - 1 || order_key(x, i) > border.key) return;
-        const double w = weight(x, s);
-        if (w >= (double)min_p) mine += units(w, s);
+    // the threshold's bin, and one to each side for the roundings at the bins' borders: only their tokens are looked at
+    const double edge = -log((double)min_p) * (OCTAVE / LN2);
+    const int b0 = edge < 2.0 ? 0 : edge < BINS ? (int)edge - 2 : BINS, b1 = b0 + 5;
+    if (b0 < BINS && (border.key == ~0ull || bin_of(key_value(border.key), s) >= b0)) {
+      u64 sum = 0;
+      const float least = edge_of(min(b1, BINS - 1), s), beyond = b0 ? edge_of(b0 - 1, s) : INFINITY;
+      for_each<T>(p, row, [&](float x, int i) {
+        if (!(x >= least && (x < beyond || b0 == 0)) || order_key(x, i) > border.key) return;
+        if (weight(x) >= (double)min_p) sum += steps(order_key(x, i));
       });
       __syncthreads();
-      const Sums v = scan(Sums{mine, 0}, per_wave);
-      if (tid == THREADS - 1) hit_s.sums = v;
+      const Sums v = scan(Sums{sum, 0}, per_wave);
+      if (tid == THREADS - 1) edge_s = v.mass;
       __syncthreads();
-      kept = (b0 ? mass[b0 - 1] : 0) + hit_s.sums.mass;
-      __syncthreads();
-      kept = max(kept, (u64)s.unit);                  // the first token stays whatever min_p is
+      kept = max((b0 ? mass[b0 - 1] : 0) + edge_s, top_steps);         // the first token stays whatever min_p is
     }
   }
-  const float u = p.uniforms[row];
-  const u64 target = 1 + min((u64)((u > 0.f ? min((double)u, 1.0) : 0.0) * (double)kept), kept - 1);
-  const Hit h = resolve(min(find_bin(mass, count, Sums{0, 0}, false, target), BINS - 1), false, target);
-  if (tid == 0) {
-    p.tokens[row] = (int)(unsigned)h.key;
-    if (p.logprobs) {
-      const float x = key_value(h.key);
-      p.logprobs[row] = (float)((x == top ? 0.0 : ((double)x - (double)top) * s.inv_t) - log((double)kept / s.unit));
-    }
-  }
+  const u64 target = u_target(kept);
+  const Hit h = resolve(min(bin_by_mass(target), BINS - 1), false, target);
+  if (tid == 0) answer(h.key, kept);
 }
 
-long row_bytes() { return MAX_SLICES * 8 + BINS * 12; }
+// Chunks per slice: what gives the busiest CU the least to do, where a slice costs its chunks and about half a chunk's time
+// for its histogram and scans.
+int chunks_of(int rows, int n) {
+  int best = 4;
+  long least = 0;
+  for (int c = 4; c >= 1; c /= 2) {
+    const long slices = (long)rows * ((n + c * CHUNK - 1) / (c * CHUNK)), per_cu = (slices + bagel_cu_count() - 1) / bagel_cu_count();
+    if (c == 4 || per_cu * (2 * c + 1) < least) best = c, least = per_cu * (2 * c + 1);
+  }
+  return best;
+}
+int slices_of(int rows, int n) { return (n + chunks_of(rows, n) * CHUNK - 1) / (chunks_of(rows, n) * CHUNK); }
 
 }  // namespace
 
 extern "C" long bagel_sample_rows_workspace_bytes(int rows, int n) {
-  return rows <= 0 || n <= 0 ? 0 : rows * row_bytes();
+  return rows <= 0 || n <= 0 ? 0 : (long)rows * slices_of(rows, n) * (sizeof(Slice) + LIST * 8 + BINS * 8);
 }
 
 extern "C" int bagel_sample_rows(const void* logits, long ld, int rows, int n, int logits_f32, const void* uniforms, const void* temperature,
                                  const void* top_k, const void* top_p, const void* min_p, void* tokens, void* logprobs,
                                  void* workspace, long workspace_bytes, void* stream) {
   BAGEL_CHECK(rows >= 0 && rows <= 65535, "bagel_sample_rows: rows=%d (at most 65535)", rows);
-  BAGEL_CHECK(n > 0 && n <= 1 << 20, "bagel_sample_rows: %d tokens (1 to 2^20)", n);
+  BAGEL_CHECK(n > 0 && n <= MAX_SLICES * CHUNK, "bagel_sample_rows: %d tokens (1 to 2^20)", n);
   BAGEL_CHECK(logits_f32 == 0 || logits_f32 == 1, "bagel_sample_rows: logits_f32=%d", logits_f32);
   if (rows == 0) return 0;
   BAGEL_CHECK(logits && uniforms && tokens && workspace, "bagel_sample_rows: null operand");
@@ -429,23 +888,25 @@ extern "C" int bagel_sample_rows(const void* logits, long ld, int rows, int n, i
   Params p;
   p.logits = logits; p.ld = ld; p.n = n;
   p.vec = (uintptr_t)logits % 16 == 0 && ld % (logits_f32 ? 4 : 8) == 0;
-  p.shift = n <= 1 << 18 ? 44 : n <= 1 << 19 ? 43 : 42;
   p.uniforms = (const float*)uniforms; p.temperature = (const float*)temperature; p.top_k = (const int*)top_k;
   p.top_p = (const float*)top_p; p.min_p = (const float*)min_p; p.tokens = (int*)tokens; p.logprobs = (float*)logprobs;
-  p.mass = (u64*)workspace;
-  p.best = p.mass + (long)rows * BINS;
-  p.count = (unsigned*)(p.best + (long)rows * MAX_SLICES);
-  // two workgroups per CU, each with at least 8192 tokens
-  p.slices = std::max(1, std::min(std::min(MAX_SLICES, 2 * bagel_cu_count() / rows), n / 8192));
+  p.slices = slices_of(rows, n);
+  const long slices = (long)rows * p.slices;
+  p.slice = (Slice*)workspace;
+  p.list = (u64*)(p.slice + slices);
+  p.bins = p.list + slices * LIST;
   const dim3 grid(p.slices, rows), block(THREADS);
+  const int c = chunks_of(rows, n);
   hipStream_t st = (hipStream_t)stream;
   if (logits_f32) {
-    hipLaunchKernelGGL(sample_top_kernel<float>, grid, block, 0, st, p);
-    hipLaunchKernelGGL(sample_histogram_kernel<float>, grid, block, 0, st, p);
+    if (c == 4) hipLaunchKernelGGL((sample_slice_kernel<float, 4>), grid, block, 0, st, p);
+    else if (c == 2) hipLaunchKernelGGL((sample_slice_kernel<float, 2>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((sample_slice_kernel<float, 1>), grid, block, 0, st, p);
     hipLaunchKernelGGL(sample_pick_kernel<float>, dim3(rows), block, 0, st, p);
   } else {
-    hipLaunchKernelGGL(sample_top_kernel<bf16>, grid, block, 0, st, p);
-    hipLaunchKernelGGL(sample_histogram_kernel<bf16>, grid, block, 0, st, p);
+    if (c == 4) hipLaunchKernelGGL((sample_slice_kernel<bf16, 4>), grid, block, 0, st, p);
+    else if (c == 2) hipLaunchKernelGGL((sample_slice_kernel<bf16, 2>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((sample_slice_kernel<bf16, 1>), grid, block, 0, st, p);
     hipLaunchKernelGGL(sample_pick_kernel<bf16>, dim3(rows), block, 0, st, p);
   }
   BAGEL_LAUNCH_CHECK();
