@@ -39,8 +39,8 @@ constexpr int FINER = 10;            // bins are added up in steps of 2^-(32 + 1
 constexpr int COUNT_SHIFT = 48;      // a slice's bin: steps (2^15 tokens stay below 2^48), and the count above them
 constexpr int SUB = 2048;            // bins of a narrowing histogram
 constexpr int CAP = 4096;            // tokens that are sorted at once
-constexpr int LIST = 1024;           // tokens that a slice lists at most
-constexpr int FEW = 1024;            // a top-k up to here is looked for in the lists first
+constexpr int LIST = 512;            // tokens that a slice lists at most
+constexpr int FEW = 512;             // a top-k up to here is looked for in the lists first
 constexpr int THREADS = 1024;
 constexpr int CHUNK = 8 * THREADS;   // logits that a workgroup loads at a time
 constexpr int MAX_SLICES = 128;      // 2^20 logits in single chunks
@@ -82,13 +82,14 @@ __device__ __forceinline__ float key_value(u64 key) {
 struct Scale {
   float top;
   double per;        // 32 log2(e) / T
+  double inverse;    // of it, or nearly
   double base;       // bin of the maximum
 };
 constexpr double LN2 = 0.69314718055994530942;
 __device__ __forceinline__ Scale make_scale(float top, float t) {
 #pragma clang fp contract(off)
   const double per = OCTAVE / LN2 / (double)t;
-  return Scale{top, per, __builtin_floor((double)top * per)};
+  return Scale{top, per, (double)t * (LN2 / OCTAVE), __builtin_floor((double)top * per)};
 }
 // Token x's bin, BINS for one that weighs nothing, and `part` = v - floor(v).  The maximum is in bin 0 even where v is no
 // number (an infinite maximum, an infinite T).
@@ -112,17 +113,16 @@ __device__ __forceinline__ float next(float x, int step) {
   return __uint_as_float(up ^ ((up >> 31) ? 0x80000000u : 0xffffffffu));
 }
 __device__ __forceinline__ float before(float x) { return next(x, -1); }
-// The smallest value in a bin up to `b`: x is in one of them just when it is not below.
+// The smallest value in a bin up to `b`: x is in one of them just when it is not below.  By a whole wave, whose lanes try the
+// values around lowest / per; the quotient is within a step or two of it.
 __device__ __forceinline__ float edge_of(int b, const Scale& s) {
 #pragma clang fp contract(off)
   if (s.top == INFINITY) return s.top;
-  const double lowest = s.base - b;
-  auto inside = [&](float x) { return (double)x * s.per >= lowest; };
   if (!(s.per > 0.0)) return -3.402823466e38f;      // an infinite T: every value is in the maximum's bin
-  float x = (float)(lowest / s.per);                // off by a step or two
-  for (int i = 0; i < 4 && x > -INFINITY && inside(x); ++i) x = next(x, -1);
-  for (int i = 0; i < 8 && x < s.top && !inside(x); ++i) x = next(x, 1);
-  return x;
+  const double lowest = s.base - b;
+  const float x = next((float)(lowest * s.inverse), (int)(threadIdx.x & 63) - 32);
+  const u64 inside = __ballot((double)x * s.per >= lowest);      // false for what lies below -inf in the bits' order: NaN
+  return __shfl(x, inside ? __ffsll(inside) - 1 : 63);
 }
 // 2^(part / 32) in steps: a cubic through its values at the four Chebyshev points of [0, 1] (7e-11 of it off at most); a sum
 // with 2^52 leaves the rounded steps in the low bits.
@@ -253,42 +253,54 @@ struct Sums {
   u64 mass;
   unsigned count;
 };
-// Inclusive scans over the workgroup's threads.
-__device__ __forceinline__ u64 wave_scan(u64 v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 m = shfl_u64(v, max(lane - o, 0));
-    if (lane >= o) v += m;
-  }
+// Inclusive scans, over a wave by DPP row shifts and broadcasts, over the workgroup through the waves' totals.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned dpp_or_0(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <typename V, typename F>
+__device__ __forceinline__ V wave_scan(V v, F moved) {
+  v += moved.template operator()<0x111, 0xf>(v);      // from the lane 1, 2, 4, 8 below in the row of 16
+  v += moved.template operator()<0x112, 0xf>(v);
+  v += moved.template operator()<0x114, 0xf>(v);
+  v += moved.template operator()<0x118, 0xf>(v);
+  v += moved.template operator()<0x142, 0xa>(v);      // the last lane of rows 0 and 2 to rows 1 and 3
+  v += moved.template operator()<0x143, 0xc>(v);      // lane 31 to the upper half
   return v;
 }
+struct Move64 {
+  template <int CTRL, int ROWS>
+  __device__ __forceinline__ u64 operator()(u64 v) const {
+    return ((u64)dpp_or_0<CTRL, ROWS>((unsigned)(v >> 32)) << 32) | dpp_or_0<CTRL, ROWS>((unsigned)v);
+  }
+};
+struct Move32 {
+  template <int CTRL, int ROWS>
+  __device__ __forceinline__ unsigned operator()(unsigned v) const { return dpp_or_0<CTRL, ROWS>(v); }
+};
+__device__ __forceinline__ u64 wave_scan(u64 v) { return wave_scan(v, Move64{}); }
+constexpr int WAVES = THREADS / 64;
 __device__ __forceinline__ u64 scan(u64 v, u64* per_wave, int stride) {
   const int wave = threadIdx.x >> 6;
   v = wave_scan(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) per_wave[wave * stride] = v;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) v += per_wave[w * stride];
+#pragma unroll
+  for (int w = 0; w < WAVES - 1; ++w) v += w < wave ? per_wave[w * stride] : 0;
   return v;
 }
 __device__ __forceinline__ Sums scan(Sums v, Sums* per_wave) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6;
+  v.mass = wave_scan(v.mass);
+  v.count = wave_scan(v.count, Move32{});
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) per_wave[wave] = v;
+  __syncthreads();
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 m = shfl_u64(v.mass, max(lane - o, 0));
-    const unsigned c = (unsigned)__shfl((int)v.count, max(lane - o, 0));
-    if (lane >= o) {
-      v.mass += m;
-      v.count += c;
-    }
-  }
-  __syncthreads();
-  if (lane == 63) per_wave[wave] = v;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) {
-    v.mass += per_wave[w].mass;
-    v.count += per_wave[w].count;
+  for (int w = 0; w < WAVES - 1; ++w) {
+    v.mass += w < wave ? per_wave[w].mass : 0;
+    v.count += w < wave ? per_wave[w].count : 0;
   }
   return v;
 }
@@ -353,7 +365,6 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
   __shared__ Sums per_wave[THREADS / 64];
   __shared__ float top_s[THREADS / 64];
   __shared__ int first, reach, fits;
-  __shared__ unsigned listed;
   const T* x = (const T*)p.logits + (long)row * p.ld;
   const int from = slice * C * CHUNK + 8 * tid;
   Raw<T> v[C];
@@ -373,7 +384,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
   const int k = row_top_k(p, row);
   const bool few = k >= 1 && k <= FEW;
   for (int b = tid; b < BINS; b += THREADS) bins[b] = 0;
-  if (tid == 0) first = 0x7fffffff, reach = BINS - 1, fits = -1, listed = 0;
+  if (tid == 0) first = 0x7fffffff, reach = BINS - 1, fits = -1;
   float top = -INFINITY;
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -452,21 +463,28 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
     }
   __syncthreads();
   const int cut = min(fits, reach);
+  unsigned listed = 0;
   if (cut >= 0) {
-    u64* list = p.list + ((long)row * p.slices + slice) * LIST;
+    // places in the list by a scan over the threads' numbers of tokens: no atomics
     const float edge = edge_of(cut, s);
     settle();
+    unsigned mine = 0;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (v[c].at(e) >= edge) {
-          const unsigned at = atomicAdd(&listed, 1u);
-          if (at < LIST) list[at] = order_key(v[c].at(e), from + c * CHUNK + e);
-        }
-    __syncthreads();
+      for (int e = 0; e < 8; ++e) mine += v[c].raw(e) >= edge ? 1 : 0;
+    const unsigned upto = (unsigned)scan((u64)mine, &per_wave->mass, sizeof(Sums) / 8);
+    u64* at = p.list + ((long)row * p.slices + slice) * LIST + (upto - mine);
+    settle();
+    if (mine && upto <= LIST)                          // always: cut is a bin that fits
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (v[c].raw(e) >= edge) *at++ = order_key(v[c].raw(e), from + c * CHUNK + e);
+    listed = min(upto, (unsigned)LIST);                                     // of the last thread: all of them, bins[cut] >> COUNT_SHIFT
   }
-  if (tid == 0) *out = Slice{order_key(top, 0), (int)min(listed, (unsigned)LIST), cut};
+  if (tid == THREADS - 1) *out = Slice{order_key(top, 0), (int)listed, cut};
 }
 
 // ---- second launch: one workgroup per row finds the token
@@ -856,21 +874,23 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
 
 // Chunks per slice: what gives the busiest CU the least to do, where a slice costs its chunks and about half a chunk's time
 // for its histogram and scans.
-int chunks_of(int rows, int n) {
-  int best = 4;
+int chunks_of(int rows, int n, int f32) {
+  const int most = f32 ? 2 : 4;        // 16 registers of logits: with twice as many, two workgroups no longer fit a CU
+  int best = most;
   long least = 0;
-  for (int c = 4; c >= 1; c /= 2) {
+  for (int c = most; c >= 1; c /= 2) {
     const long slices = (long)rows * ((n + c * CHUNK - 1) / (c * CHUNK)), per_cu = (slices + bagel_cu_count() - 1) / bagel_cu_count();
-    if (c == 4 || per_cu * (2 * c + 1) < least) best = c, least = per_cu * (2 * c + 1);
+    if (c == most || per_cu * (2 * c + 1) < least) best = c, least = per_cu * (2 * c + 1);
   }
   return best;
 }
-int slices_of(int rows, int n) { return (n + chunks_of(rows, n) * CHUNK - 1) / (chunks_of(rows, n) * CHUNK); }
+int slices_of(int n, int chunks) { return (n + chunks * CHUNK - 1) / (chunks * CHUNK); }
+long workspace_of(int rows, int n, int f32) { return (long)rows * slices_of(n, chunks_of(rows, n, f32)) * (sizeof(Slice) + LIST * 8 + BINS * 8); }
 
 }  // namespace
 
 extern "C" long bagel_sample_rows_workspace_bytes(int rows, int n) {
-  return rows <= 0 || n <= 0 ? 0 : (long)rows * slices_of(rows, n) * (sizeof(Slice) + LIST * 8 + BINS * 8);
+  return rows <= 0 || n <= 0 ? 0 : std::max(workspace_of(rows, n, 0), workspace_of(rows, n, 1));
 }
 
 extern "C" int bagel_sample_rows(const void* logits, long ld, int rows, int n, int logits_f32, const void* uniforms, const void* temperature,
@@ -890,17 +910,16 @@ extern "C" int bagel_sample_rows(const void* logits, long ld, int rows, int n, i
   p.vec = (uintptr_t)logits % 16 == 0 && ld % (logits_f32 ? 4 : 8) == 0;
   p.uniforms = (const float*)uniforms; p.temperature = (const float*)temperature; p.top_k = (const int*)top_k;
   p.top_p = (const float*)top_p; p.min_p = (const float*)min_p; p.tokens = (int*)tokens; p.logprobs = (float*)logprobs;
-  p.slices = slices_of(rows, n);
+  const int c = chunks_of(rows, n, logits_f32);
+  p.slices = slices_of(n, c);
   const long slices = (long)rows * p.slices;
   p.slice = (Slice*)workspace;
   p.list = (u64*)(p.slice + slices);
   p.bins = p.list + slices * LIST;
   const dim3 grid(p.slices, rows), block(THREADS);
-  const int c = chunks_of(rows, n);
   hipStream_t st = (hipStream_t)stream;
   if (logits_f32) {
-    if (c == 4) hipLaunchKernelGGL((sample_slice_kernel<float, 4>), grid, block, 0, st, p);
-    else if (c == 2) hipLaunchKernelGGL((sample_slice_kernel<float, 2>), grid, block, 0, st, p);
+    if (c == 2) hipLaunchKernelGGL((sample_slice_kernel<float, 2>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((sample_slice_kernel<float, 1>), grid, block, 0, st, p);
     hipLaunchKernelGGL(sample_pick_kernel<float>, dim3(rows), block, 0, st, p);
   } else {
