@@ -213,39 +213,59 @@ __device__ __forceinline__ void wave_sort(u64& key) {
   wave_sort_step<64, 32>(key);
 }
 
-// Eight logits from index i on (a multiple of 8), -inf behind the row's end.
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4_;
+// Logits of a chunk as they are loaded.  settle(): what was made of them so far is not kept in registers.
 template <typename T>
-__device__ __forceinline__ void load8(const Params& p, const T* row, int i, float (&v)[8]) {
-  if (p.vec && i + 8 <= p.n) {
-    if constexpr (sizeof(T) == 2) {
-      const bf16x8 w = *(const bf16x8*)(row + i);
+struct Raw;
+template <>
+struct Raw<bf16> {
+  u32x4_ w;
+  __device__ __forceinline__ float raw(int e) const { return __uint_as_float(e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16); }
+  __device__ __forceinline__ float at(int e) const { return clean(raw(e)); }
+  __device__ __forceinline__ void settle() { asm volatile("" : "+v"(w)); }
+};
+template <>
+struct Raw<float> {
+  f32x4 w[2];
+  __device__ __forceinline__ float raw(int e) const { return w[e / 4][e % 4]; }
+  __device__ __forceinline__ float at(int e) const { return clean(raw(e)); }
+  __device__ __forceinline__ void settle() { asm volatile("" : "+v"(w[0]), "+v"(w[1])); }
+};
+
+// A row's chunk of eight logits from index i on (a multiple of 8), -inf behind the row's end.
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const Params& p, const T* row, int i) {
+  if (p.vec && i + 8 <= p.n) return *(const Raw<T>*)(row + i);
+  T w[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = clean((float)w[e]);
-    } else {
-      const f32x4 a = *(const f32x4*)(row + i), b = *(const f32x4*)(row + i + 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = clean(a[e]);
-        v[4 + e] = clean(b[e]);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = i + e < p.n ? clean((float)row[i + e]) : -INFINITY;
-  }
+  for (int e = 0; e < 8; ++e) w[e] = i + e < p.n ? row[i + e] : (T)-INFINITY;
+  return __builtin_bit_cast(Raw<T>, w);
 }
-// f(value, index) for this thread's share of a whole row, four loads in flight.
+// f(value, index) for this thread's share of a whole row's logits in [least, beyond) - a NaN for beyond: no upper end -, four
+// loads in flight.
 template <typename T, typename F>
-__device__ __forceinline__ void for_each(const Params& p, int row, F f) {
+__device__ __forceinline__ void for_range(const Params& p, int row, float least, float beyond, F f) {
   const T* x = (const T*)p.logits + (long)row * p.ld;
-  for (int i0 = 0; i0 < p.n; i0 += 4 * CHUNK) {
-    float v[4][8];
+  constexpr int N = 4;
+  for (int i0 = 8 * (int)threadIdx.x; i0 < p.n; i0 += N * CHUNK) {
+    Raw<T> v[N];
+    if (p.vec && i0 + (N - 1) * CHUNK + 8 <= p.n) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) load8(p, x, i0 + c * CHUNK + 8 * (int)threadIdx.x, v[c]);
+      for (int c = 0; c < N; ++c) v[c] = *(const Raw<T>*)(x + i0 + c * CHUNK);
+    } else {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < N; ++c) v[c] = load_raw(p, x, i0 + c * CHUNK);
+    }
+    // first which, then f: few lanes have one at the same place, and what f waits for is waited for once per round
+    unsigned hits = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f(v[c][e], i0 + c * CHUNK + 8 * (int)threadIdx.x + e);
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) hits |= (unsigned)(v[c].raw(e) >= least && !(v[c].raw(e) >= beyond)) << (8 * c + e);
+    for (; hits; hits &= hits - 1) {
+      const int bit = __ffs(hits) - 1, i = i0 + bit / 8 * CHUNK + bit % 8;
+      f((float)x[i], i);
+    }
   }
 }
 
@@ -338,25 +358,6 @@ __device__ __forceinline__ int row_top_k(const Params& p, int row) {
   return k >= 1 && k < p.n ? k : 0;
 }
 
-typedef __attribute__((ext_vector_type(4))) unsigned u32x4_;
-// Logits of a chunk as they are loaded.  settle(): what was made of them so far is not kept in registers.
-template <typename T>
-struct Raw;
-template <>
-struct Raw<bf16> {
-  u32x4_ w;
-  __device__ __forceinline__ float raw(int e) const { return __uint_as_float(e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16); }
-  __device__ __forceinline__ float at(int e) const { return clean(raw(e)); }
-  __device__ __forceinline__ void settle() { asm volatile("" : "+v"(w)); }
-};
-template <>
-struct Raw<float> {
-  f32x4 w[2];
-  __device__ __forceinline__ float raw(int e) const { return w[e / 4][e % 4]; }
-  __device__ __forceinline__ float at(int e) const { return clean(raw(e)); }
-  __device__ __forceinline__ void settle() { asm volatile("" : "+v"(w[0]), "+v"(w[1])); }
-};
-
 // ---- first launch: a workgroup per slice of C chunks
 template <typename T, int C>
 __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
@@ -373,12 +374,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
     for (int c = 0; c < C; ++c) v[c] = *(const Raw<T>*)(x + from + c * CHUNK);
   } else {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      T w[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = from + c * CHUNK + e < p.n ? x[from + c * CHUNK + e] : (T)-INFINITY;
-      v[c] = __builtin_bit_cast(Raw<T>, w);
-    }
+    for (int c = 0; c < C; ++c) v[c] = load_raw(p, x, from + c * CHUNK);
   }
   const float t = row_temperature(p, row);
   const int k = row_top_k(p, row);
@@ -590,22 +586,37 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
     const unsigned at = atomicAdd(&gathered, 1u);
     if (at < CAP) work[at] = key;
   };
+  // work[0 ... len) ascending: a bitonic network whose steps inside 64 keys run in a wave's registers
   auto sort = [&](int len) {
-    int size = 2;
+    int size = 64;
     while (size < len) size *= 2;
     __syncthreads();
     for (int i = len + tid; i < size; i += THREADS) work[i] = ~0ull;
-    for (int q = 2; q <= size; q *= 2)
-      for (int j = q / 2; j > 0; j /= 2) {
+    __syncthreads();
+    const int wave = tid >> 6, lane = tid & 63;
+    for (int at = wave * 64; at < size; at += THREADS) {
+      const u64 turned = at & 64 ? ~0ull : 0;                // descending: ascending in the complement
+      u64 key = work[at + lane] ^ turned;
+      wave_sort(key);
+      work[at + lane] = key ^ turned;
+    }
+    for (int q = 128; q <= size; q *= 2) {
+      for (int j = q / 2; j >= 64; j /= 2) {
         __syncthreads();
-        for (int i = tid; i < size; i += THREADS) {
-          const int o = i ^ j;
-          if (o > i) {
-            const u64 a = work[i], b = work[o];
-            if ((a > b) == ((i & q) == 0)) work[i] = b, work[o] = a;
-          }
+        for (int t = tid; t < size / 2; t += THREADS) {
+          const int i = 2 * t - (t & (j - 1)), o = i + j;
+          const u64 a = work[i], b = work[o];
+          if ((a > b) == ((i & q) == 0)) work[i] = b, work[o] = a;
         }
       }
+      __syncthreads();
+      for (int at = wave * 64; at < size; at += THREADS) {
+        const u64 turned = at & q ? ~0ull : 0;
+        u64 key = work[at + lane] ^ turned;
+        wave_sort_step<64, 32>(key);
+        work[at + lane] = key ^ turned;
+      }
+    }
     __syncthreads();
   };
   constexpr int EACH = CAP / THREADS;        // neighbours per thread in the sorted order
@@ -703,33 +714,33 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
     __syncthreads();
     return b;
   };
-  if (few && enough && listed <= CAP) {
-    float edge = -INFINITY;
-    if (listed > 64) {
-      // of the slices' first k only those in the bins of the row's first k
-      for (int b = tid; b < BINS; b += THREADS) mass[b] = 0;
-      __syncthreads();
-      for_listed([&](u64 key) {
-        const int b = bin_of(key_value(key), s);
-        if (b < BINS) atomicAdd(&mass[b], 1ull);
-      });
-      prefix<BINS>(mass, per_wave);
-      const int b = find(BINS, [&](int b) { return (b == 0 || mass[b - 1] < (u64)k) && mass[b] >= (u64)k; });
-      if (b < BINS) edge = edge_of(b, s);
-    }
-    for_listed([&](u64 key) {
-      if (key_value(key) >= edge) put(key);
-    });
+  if (few && enough) {
+    // of the slices' first k only those in the bins of the row's first k (or all, where that many weigh nothing)
+    for (int b = tid; b < BINS; b += THREADS) mass[b] = 0;
     __syncthreads();
-    finish((int)min(gathered, (unsigned)CAP), 0);
-    return;
+    for_listed([&](u64 key) {
+      const int b = bin_of(key_value(key), s);
+      if (b < BINS) atomicAdd(&mass[b], 1ull);
+    });
+    prefix<BINS>(mass, per_wave);
+    const int b = min(find(BINS, [&](int b) { return (b == 0 || mass[b - 1] < (u64)k) && mass[b] >= (u64)k; }), BINS - 1);
+    if (mass[b] <= CAP) {
+      const float edge = edge_of(b, s);
+      for_listed([&](u64 key) {
+        if (key_value(key) >= edge) put(key);
+      });
+      __syncthreads();
+      finish((int)min(gathered, (unsigned)CAP), 0);
+      return;
+    }
+    __syncthreads();
   }
 
   // the row's histogram: the slices' or, where the lists of a top-k did not do and weights were left out, made here
   if (few) {
     for (int b = tid; b < BINS; b += THREADS) mass[b] = 0, count[b] = 0;
     __syncthreads();
-    for_each<T>(p, row, [&](float x, int) {
+    for_range<T>(p, row, edge_of(BINS - 1, s), __builtin_nanf(""), [&](float x, int) {
       double part;
       const int b = bin_of(x, s, part);
       if (b < BINS) {
@@ -769,12 +780,7 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
     auto reached = [&](u64 m, unsigned c) {
       return by_count ? (u64)(base.count + inner.count + c) >= target : base.mass + scaled(inner.mass + m, bin, table) >= target;
     };
-    const float least = edge_of(bin, s), beyond = bin ? edge_of(bin - 1, s) : INFINITY;
-    auto in_bin = [&](float x, int i, u64& key) {
-      if (!(x >= least && (x < beyond || bin == 0))) return false;
-      key = order_key(x, i);
-      return key >= low && key <= high;
-    };
+    const float least = edge_of(bin, s), beyond = bin ? edge_of(bin - 1, s) : __builtin_nanf("");
     auto part_steps = [&](u64 key) {
       double part;
       place(key, part);
@@ -784,9 +790,9 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
       __syncthreads();
       for (int b = tid; b < SUB; b += THREADS) sub_mass[b] = 0, sub_count[b] = 0;
       __syncthreads();
-      for_each<T>(p, row, [&](float x, int i) {
-        u64 key;
-        if (!in_bin(x, i, key)) return;
+      for_range<T>(p, row, least, beyond, [&](float x, int i) {
+        const u64 key = order_key(x, i);
+        if (key < low || key > high) return;
         const int b = (int)((key - low) >> sh);
         atomicAdd(&sub_count[b], 1u);
         atomicAdd(&sub_mass[b], part_steps(key));
@@ -804,12 +810,13 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
     __syncthreads();
     if (tid == 0) gathered = 0;
     __syncthreads();
-    auto gather = [&](float x, int i) {
-      u64 key;
-      if (in_bin(x, i, key)) put(key);
+    auto gather = [&](u64 key) {
+      if (key >= low && key <= high) put(key);
     };
-    if (bin <= lowest_cut) for_listed([&](u64 key) { gather(key_value(key), (int)(unsigned)key); });
-    else for_each<T>(p, row, gather);
+    if (bin <= lowest_cut) for_listed([&](u64 key) {
+      if (key_value(key) >= least && !(key_value(key) >= beyond)) gather(key);
+    });
+    else for_range<T>(p, row, least, beyond, [&](float x, int i) { gather(order_key(x, i)); });
     __syncthreads();
     const int len = (int)min(gathered, (unsigned)CAP);
     sort(len);
@@ -855,11 +862,14 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
     const int b0 = edge < 2.0 ? 0 : edge < BINS ? (int)edge - 2 : BINS, b1 = b0 + 5;
     if (b0 < BINS && (border.key == ~0ull || bin_of(key_value(border.key), s) >= b0)) {
       u64 sum = 0;
-      const float least = edge_of(min(b1, BINS - 1), s), beyond = b0 ? edge_of(b0 - 1, s) : INFINITY;
-      for_each<T>(p, row, [&](float x, int i) {
-        if (!(x >= least && (x < beyond || b0 == 0)) || order_key(x, i) > border.key) return;
-        if (weight(x) >= (double)min_p) sum += steps(order_key(x, i));
+      const float least = edge_of(min(b1, BINS - 1), s), beyond = b0 ? edge_of(b0 - 1, s) : __builtin_nanf("");
+      auto add = [&](u64 key) {
+        if (key <= border.key && weight(key_value(key)) >= (double)min_p) sum += steps(key);
+      };
+      if (b1 <= lowest_cut) for_listed([&](u64 key) {
+        if (key_value(key) >= least && !(key_value(key) >= beyond)) add(key);
       });
+      else for_range<T>(p, row, least, beyond, [&](float x, int i) { add(order_key(x, i)); });
       __syncthreads();
       const Sums v = scan(Sums{sum, 0}, per_wave);
       if (tid == THREADS - 1) edge_s = v.mass;
