@@ -152,8 +152,7 @@ int launch_append(const AppendParams& p, hipStream_t st) {
 // the matrix product (an error of 2^-9 of each weight, which the output's own rounding to bf16 exceeds).
 // An e4m3 value is a bf16 value: keys and values are widened exactly, the scales enter in fp32.
 //
-// One workgroup = four waves that take turns at the chunk's tiles, each with its own running softmax; two tiles of every
-// wave are in flight while it computes.  A row with more keys than one chunk is split over workgroups; each leaves an
+// One workgroup = four waves that take turns at the chunk's tiles, each with its own running softmax.  A row with more keys than one chunk is split over workgroups; each leaves an
 // unnormalised partial (sums in fp32) and the last one to finish joins them in chunk order.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int WAVES = 4;
@@ -196,11 +195,12 @@ __device__ __forceinline__ float column_sum(float v) {
 }
 
 template <int D, bool F8>
-__global__ __launch_bounds__(64 * WAVES, 2) void paged_attention_kernel(AttendParams p) {
+__global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendParams p) {
   constexpr int ITEM = F8 ? 1 : 2;
   constexpr int SUB = 256 / (D * ITEM);        // blocks of 32 keys per tile: a tile is 8 KB of keys and 8 KB of values
   constexpr int TK = 32 * SUB;                 // keys per tile
-  constexpr int KC = D * ITEM / 64;            // 16-byte loads of a key row per lane
+  constexpr int CH = D * ITEM / 16;            // 16-byte pieces of a key row
+  constexpr int RPI = 64 / CH;                 // key rows that one load instruction of a wave covers, whole
   constexpr int KM = D / 32;                   // matrix instructions per 16 keys of S^T
   constexpr int ND = D / 16;                   // d's per lane of a value row
   constexpr int VW = ND * ITEM / 4;            // dwords per lane of a value row
@@ -226,55 +226,78 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attention_kernel(AttendPa
   if (c >= nsplit) return;
   const int begin = c * chunk, end = min(len - begin, chunk) + begin;
 
-  __shared__ float o_s[WAVES][16][D + 4];
+  union Shared {
+    u32x4 keys[WAVES][8 * 64];                 // each wave's tile of keys
+    float o[WAVES][16][D + 4];
+  };
+  __shared__ Shared lds;
   __shared__ float m_s[WAVES][16], l_s[WAVES][16];
   __shared__ unsigned ticket_s;
 
   const int* table = p.table + row * p.table_stride;
   const int mask = (1 << p.page_shift) - 1;
   const int last_page = (len - 1) >> p.page_shift;
-  const int kr = 8 * (n >> 2) + (n & 3);       // this lane's key row (of tile 0) among 32
-  const char* kbase = p.k.base + kvh * p.k.head + 16 * g;
+  const char* kbase = p.k.base + kvh * p.k.head + (long)(lane / CH) * p.k.slot;
   const char* vbase = p.v.base + kvh * p.v.head + n * (ND * ITEM);
+  u32x4* keys = lds.keys[wave];
 
-  struct Ids {
-    int k[SUB], v[SUB];
+  // Pieces of a key row lie in LDS exchanged by XOR with `turn` of the row, so that the eight lanes that read the same piece
+  // of eight rows at once (keys 0 ... 3 and 8 ... 11, or 4 more) find them in eight different places of 128 bytes.
+  auto turn = [](int key) {
+    const int r = 4 * ((key >> 3) & 1) + (key & 3);
+    return CH == 4 ? r >> 1 : r;
   };
+
   struct Tile {
-    u32x4 k[SUB][2][KC];
     unsigned v[SUB][8][VW];
   };
-  // page ids of the tile at key k0; a page id outside the pool is not followed: the row's output says so instead
-  auto load_ids = [&](Ids& x, int k0) {
+  // Page ids of the tile at key k0, one per lane group and block of 32: that of keys 8 g ... 8 g + 7, of which no page holds a
+  // part.  A page id outside the pool is not followed: the row's output says so instead.
+  auto load_ids = [&](int (&ids)[SUB], int k0) {
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) ids[s] = table[min((k0 + 32 * s + 8 * g) >> p.page_shift, last_page)];
+  };
+  auto check_ids = [&](int (&ids)[SUB]) {
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-      x.k[s] = table[min((k0 + 32 * s + (kr & ~7)) >> p.page_shift, last_page)];
-      x.v[s] = table[min((k0 + 32 * s + 8 * g) >> p.page_shift, last_page)];
+      const bool none = (unsigned)ids[s] >= (unsigned)p.num_pages;
+      bad |= none;
+      ids[s] = none ? 0 : ids[s];
     }
   };
-  auto load_tile = [&](Tile& x, const Ids& ids, int k0) {
+  // Keys go to LDS without passing a register, in whole rows and past the caches (each is read once).
+  auto load_keys = [&](const int (&ids)[SUB], int k0) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the tile before has been read
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // the groups of eight keys of this instruction's rows: one, or two with 16 rows
+      auto row0 = [&](int group) {
+        const long page = __builtin_amdgcn_readlane(ids[group / 4], 16 * (group % 4));
+        return page * p.k.page + (long)((k0 + 8 * group) & mask) * p.k.slot;
+      };
+      const int first = i * RPI;                              // of the tile
+      long at = row0(first / 8) + (long)(first % 8) * p.k.slot;
+      if constexpr (RPI == 16) at = lane < 32 ? at : row0(first / 8 + 1) - 8 * p.k.slot;      // kbase counts rows from the first
+      const char* src = kbase + at + 16 * ((lane % CH) ^ turn(first + lane / CH));
+      __builtin_amdgcn_global_load_lds(GLOBAL_PTR(src), LDS_PTR(keys + 64 * i), 16, 0, 2);
+    }
+  };
+  auto load_values = [&](Tile& x, const int (&ids)[SUB], int k0) {
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-      const bool kb = (unsigned)ids.k[s] >= (unsigned)p.num_pages, vb = (unsigned)ids.v[s] >= (unsigned)p.num_pages;
-      bad |= kb | vb;
-      const char* kp = kbase + (long)(kb ? 0 : ids.k[s]) * p.k.page + (long)((k0 + 32 * s + kr) & mask) * p.k.slot;
-      const char* vp = vbase + (long)(vb ? 0 : ids.v[s]) * p.v.page + (long)((k0 + 32 * s + 8 * g) & mask) * p.v.slot;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < KC; ++i) x.k[s][t][i] = *(const u32x4*)(kp + 4 * t * p.k.slot + 64 * i);
+      const char* vp = vbase + (long)ids[s] * p.v.page + (long)((k0 + 32 * s + 8 * g) & mask) * p.v.slot;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if constexpr (VW == 4) {
-          const u32x4 w = *(const u32x4*)(vp + e * p.v.slot);
+          const u32x4 w = __builtin_nontemporal_load((const u32x4*)(vp + e * p.v.slot));
 #pragma unroll
           for (int i = 0; i < 4; ++i) x.v[s][e][i] = w[i];
         } else if constexpr (VW == 2) {
-          const u32x2 w = *(const u32x2*)(vp + e * p.v.slot);
+          const u32x2 w = __builtin_nontemporal_load((const u32x2*)(vp + e * p.v.slot));
           x.v[s][e][0] = w[0];
           x.v[s][e][1] = w[1];
         } else {
-          x.v[s][e][0] = *(const unsigned*)(vp + e * p.v.slot);
+          x.v[s][e][0] = __builtin_nontemporal_load((const unsigned*)(vp + e * p.v.slot));
         }
       }
     }
@@ -295,39 +318,29 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attention_kernel(AttendPa
   for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = -INFINITY, l_run = 0.f;        // l_run: this lane's keys only
 
-  auto compute = [&](Tile& x, int k0) {
-    float s[SUB][8];
+  typedef float Scores[SUB][8];
+  auto scores = [&](Scores& s) {
 #pragma unroll
     for (int b = 0; b < SUB; ++b)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int key = 32 * b + 8 * (n >> 2) + 4 * t + (n & 3);      // this lane's row
 #pragma unroll
-        for (int j = 0; j < KM; ++j) {
-          bf16x8 kf;
+        for (int c = 0; c < CH / 4; ++c) {
+          const u32x4 w = keys[key * CH + ((4 * c + g) ^ turn(key))];
           if constexpr (F8) {
-            const u32x4 w = x.k[b][t][j / 2];
-            kf = widen8(w[2 * (j % 2)], w[2 * (j % 2) + 1]);
+            a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(w[0], w[1]), q[2 * c], a, 0, 0, 0);
+            a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(w[2], w[3]), q[2 * c + 1], a, 0, 0, 0);
           } else {
-            kf = __builtin_bit_cast(bf16x8, x.k[b][t][j]);
+            a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), q[c], a, 0, 0, 0);
           }
-          a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[j], a, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[b][4 * t + i] = a[i] * scale;
       }
-    if (k0 + TK > end) {
-      // keys behind the end: their scores are replaced, and their values cleared (0 x NaN is NaN)
-#pragma unroll
-      for (int b = 0; b < SUB; ++b)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (k0 + 32 * b + 8 * g + e >= end) {
-            s[b][e] = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < VW; ++i) x.v[b][e][i] = 0;
-          }
-    }
+  };
+  auto add_values = [&](const Tile& x, Scores& s) {
     float mx = s[0][0];
 #pragma unroll
     for (int b = 0; b < SUB; ++b)
@@ -367,28 +380,48 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attention_kernel(AttendPa
     }
   };
 
-  Ids ia, ib;
-  Tile ta, tb;
+  // A wave's next keys are requested as soon as its scores are there, its next values after their product; the other waves
+  // of the SIMD compute meanwhile.  No load of the loop is conditional: the waits are counted, and a load that may have been
+  // left out would have to be waited for as if it were.
   constexpr int STEP = WAVES * TK;
   int k0 = begin + wave * TK;
-  if (k0 < end) load_ids(ia, k0);
-  if (k0 + STEP < end) load_ids(ib, k0 + STEP);
-  if (k0 < end) load_tile(ta, ia, k0);
-  if (k0 + 2 * STEP < end) load_ids(ia, k0 + 2 * STEP);
-  if (k0 + STEP < end) load_tile(tb, ib, k0 + STEP);
-  if (k0 + 3 * STEP < end) load_ids(ib, k0 + 3 * STEP);
-  for (; k0 < end; k0 += 2 * STEP) {
-    compute(ta, k0);
-    if (k0 + 2 * STEP < end) load_tile(ta, ia, k0 + 2 * STEP);
-    if (k0 + 4 * STEP < end) load_ids(ia, k0 + 4 * STEP);
-    if (k0 + STEP < end) compute(tb, k0 + STEP);
-    if (k0 + 3 * STEP < end) load_tile(tb, ib, k0 + 3 * STEP);
-    if (k0 + 5 * STEP < end) load_ids(ib, k0 + 5 * STEP);
+  if (k0 < end) {
+    int ids[SUB], next[SUB];
+    Tile x;
+    Scores s;
+    load_ids(ids, k0);
+    load_ids(next, k0 + STEP);
+    check_ids(ids);
+    load_keys(ids, k0);
+    load_values(x, ids, k0);
+    for (; k0 + STEP < end; k0 += STEP) {
+      check_ids(next);
+#pragma unroll
+      for (int b = 0; b < SUB; ++b) ids[b] = next[b];
+      load_ids(next, k0 + 2 * STEP);
+      scores(s);
+      load_keys(ids, k0 + STEP);
+      add_values(x, s);
+      load_values(x, ids, k0 + STEP);
+    }
+    scores(s);
+    // keys behind the end: their scores are replaced, and their values cleared (0 x NaN is NaN)
+#pragma unroll
+    for (int b = 0; b < SUB; ++b)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (k0 + 32 * b + 8 * g + e >= end) {
+          s[b][e] = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < VW; ++i) x.v[b][e][i] = 0;
+        }
+    add_values(x, s);
   }
 
   // ---- join the waves
   l_run = column_sum(l_run);
   if (__any(bad)) l_run = __builtin_nanf("");
+  __syncthreads();                             // the last keys have been read everywhere
   if (g == 0) {
     m_s[wave][n] = m_run;
     l_s[wave][n] = l_run;
@@ -396,7 +429,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attention_kernel(AttendPa
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int dd = 0; dd < ND; ++dd) o_s[wave][n][ND * (4 * g + i) + dd] = acc[dd][i];
+    for (int dd = 0; dd < ND; ++dd) lds.o[wave][n][ND * (4 * g + i) + dd] = acc[dd][i];
   __syncthreads();
   const float vscale = F8 ? p.v.scale[kvh] : 1.0f;
   const long pair = ((long)row * p.Hkv + kvh) * ((rep + 15) / 16) + hb;
@@ -411,7 +444,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attention_kernel(AttendPa
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       const float f = __builtin_amdgcn_exp2f(m_s[w][h] - mx);
-      o += o_s[w][h][d] * f;
+      o += lds.o[w][h][d] * f;
       l += l_s[w][h] * f;
     }
     if (nsplit == 1) {
