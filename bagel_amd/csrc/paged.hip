@@ -156,7 +156,15 @@ int launch_append(const AppendParams& p, hipStream_t st) {
 // unnormalised partial (sums in fp32) and the last one to finish joins them in chunk order.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int WAVES = 4;
-constexpr int MAX_SPLITS = 128;
+constexpr int JOIN = 16;             // partials that are joined at once
+constexpr int MAX_SPLITS = 8 * JOIN;
+constexpr int TICKETS = 16;          // per (row, kv head, head block): one for all chunks or groups of them, eight for the groups
+
+// Blocks of 32 keys per tile: 8 KB of keys and as much of values, half of that for the shortest rows.
+template <int D, bool F8>
+constexpr int tile_blocks() {
+  return D * (F8 ? 1 : 2) == 256 ? 1 : 2;
+}
 
 struct AttendParams {
   const bf16* Q;
@@ -168,8 +176,9 @@ struct AttendParams {
   const int* kv_lens;
   bf16* O;
   long ldo;
-  float* part;           // [rows][Hkv][head blocks][splits][heads in the block][D + 2]
-  unsigned* tickets;     // [rows][Hkv][head blocks], zero on entry, left zero
+  float* part;           // [rows][Hkv][head blocks][splits][heads in the block][D] sums
+  float2* stats;         // [rows][Hkv][head blocks][splits][heads in the block] maximum, weight
+  unsigned* tickets;     // [rows][Hkv][head blocks][TICKETS], zero on entry, left zero
   int Hq, Hkv, chunk;
   float scale_log2;
 };
@@ -197,14 +206,14 @@ __device__ __forceinline__ float column_sum(float v) {
 template <int D, bool F8>
 __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendParams p) {
   constexpr int ITEM = F8 ? 1 : 2;
-  constexpr int SUB = 256 / (D * ITEM);        // blocks of 32 keys per tile: a tile is 8 KB of keys and 8 KB of values
+  constexpr int SUB = tile_blocks<D, F8>();    // blocks of 32 keys per tile
   constexpr int TK = 32 * SUB;                 // keys per tile
   constexpr int CH = D * ITEM / 16;            // 16-byte pieces of a key row
   constexpr int RPI = 64 / CH;                 // key rows that one load instruction of a wave covers, whole
+  constexpr int LOADS = TK / RPI;              // such instructions per tile
   constexpr int KM = D / 32;                   // matrix instructions per 16 keys of S^T
   constexpr int ND = D / 16;                   // d's per lane of a value row
   constexpr int VW = ND * ITEM / 4;            // dwords per lane of a value row
-  constexpr int PW = D + 2;                    // floats of a partial: sums, maximum, weight
   const int row = blockIdx.z, kvh = blockIdx.y % p.Hkv, hb = blockIdx.y / p.Hkv, c = blockIdx.x;
   const int rep = p.Hq / p.Hkv, h0 = hb * 16, nh = min(16, rep - h0);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -227,7 +236,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
   const int begin = c * chunk, end = min(len - begin, chunk) + begin;
 
   union Shared {
-    u32x4 keys[WAVES][8 * 64];                 // each wave's tile of keys
+    u32x4 keys[WAVES][LOADS * 64];             // each wave's tile of keys
     float o[WAVES][16][D + 4];
   };
   __shared__ Shared lds;
@@ -237,6 +246,8 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
   const int* table = p.table + row * p.table_stride;
   const int mask = (1 << p.page_shift) - 1;
   const int last_page = (len - 1) >> p.page_shift;
+  // Whole rows of 128 bytes and more pass the caches by (each is read once); two rows of 64 share a line.
+  constexpr bool PAST = CH >= 8;
   const char* kbase = p.k.base + kvh * p.k.head + (long)(lane / CH) * p.k.slot;
   const char* vbase = p.v.base + kvh * p.v.head + n * (ND * ITEM);
   u32x4* keys = lds.keys[wave];
@@ -265,11 +276,11 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
       ids[s] = none ? 0 : ids[s];
     }
   };
-  // Keys go to LDS without passing a register, in whole rows and past the caches (each is read once).
+  // Keys go to LDS without passing a register, in whole rows.
   auto load_keys = [&](const int (&ids)[SUB], int k0) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the tile before has been read
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < LOADS; ++i) {
       // the groups of eight keys of this instruction's rows: one, or two with 16 rows
       auto row0 = [&](int group) {
         const long page = __builtin_amdgcn_readlane(ids[group / 4], 16 * (group % 4));
@@ -279,7 +290,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
       long at = row0(first / 8) + (long)(first % 8) * p.k.slot;
       if constexpr (RPI == 16) at = lane < 32 ? at : row0(first / 8 + 1) - 8 * p.k.slot;      // kbase counts rows from the first
       const char* src = kbase + at + 16 * ((lane % CH) ^ turn(first + lane / CH));
-      __builtin_amdgcn_global_load_lds(GLOBAL_PTR(src), LDS_PTR(keys + 64 * i), 16, 0, 2);
+      __builtin_amdgcn_global_load_lds(GLOBAL_PTR(src), LDS_PTR(keys + 64 * i), 16, 0, PAST ? 2 : 0);
     }
   };
   auto load_values = [&](Tile& x, const int (&ids)[SUB], int k0) {
@@ -297,7 +308,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
           x.v[s][e][0] = w[0];
           x.v[s][e][1] = w[1];
         } else {
-          x.v[s][e][0] = __builtin_nontemporal_load((const unsigned*)(vp + e * p.v.slot));
+          x.v[s][e][0] = *(const unsigned*)(vp + e * p.v.slot);
         }
       }
     }
@@ -432,66 +443,100 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
     for (int dd = 0; dd < ND; ++dd) lds.o[wave][n][ND * (4 * g + i) + dd] = acc[dd][i];
   __syncthreads();
   const float vscale = F8 ? p.v.scale[kvh] : 1.0f;
+  // two neighbouring d's of a head per thread
+  auto finish = [&](int i, float o0, float o1, float l) {
+    const bf16x2 o = {(bf16)(o0 / l * vscale), (bf16)(o1 / l * vscale)};
+    *(bf16x2*)(orow + 2 * i) = o;
+  };
   const long pair = ((long)row * p.Hkv + kvh) * ((rep + 15) / 16) + hb;
   // partials of all head blocks of a (row, kv head) lie together: rep heads of `splits_max` chunks
-  float* part = p.part + (((long)row * p.Hkv + kvh) * rep + h0) * splits_max * PW;
-  for (int i = tid; i < nh * D; i += 64 * WAVES) {
-    const int h = i / D, d = i % D;
+  const long block = (((long)row * p.Hkv + kvh) * rep + h0) * splits_max;
+  unsigned long long* part = (unsigned long long*)(p.part + block * D);
+  unsigned long long* stats = (unsigned long long*)(p.stats + block);
+  // Partials pass between workgroups on different XCDs by the same forms as in decode_attention.hip: agent-scope stores and
+  // loads (written through, read past the CU's cache), every store complete before the ticket is taken.
+  auto put = [&](unsigned long long* at, float a, float b) {
+    __hip_atomic_store(at, ((unsigned long long)__float_as_uint(b) << 32) | __float_as_uint(a), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  auto get = [&](const unsigned long long* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  auto low = [](unsigned long long v) { return __uint_as_float((unsigned)v); };
+  auto high = [](unsigned long long v) { return __uint_as_float((unsigned)(v >> 32)); };
+  for (int i = tid; i < nh * D / 2; i += 64 * WAVES) {
+    const int h = i / (D / 2), d = 2 * (i % (D / 2));
     float mx = m_s[0][h];                                   // wave 0 always had a tile
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) mx = fmaxf(mx, m_s[w][h]);
-    float o = 0.f, l = 0.f;
+    float o0 = 0.f, o1 = 0.f, l = 0.f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       const float f = __builtin_amdgcn_exp2f(m_s[w][h] - mx);
-      o += lds.o[w][h][d] * f;
+      o0 += lds.o[w][h][d] * f;
+      o1 += lds.o[w][h][d + 1] * f;
       l += l_s[w][h] * f;
     }
     if (nsplit == 1) {
-      orow[i] = (bf16)(o / l * vscale);
+      finish(i, o0, o1, l);
     } else {
-      // Partials pass between workgroups on different XCDs by the same forms as in decode_attention.hip: agent-scope
-      // stores and loads (written through, read past the CU's cache), every store complete before the ticket is taken.
-      float* mine = part + ((long)c * nh + h) * PW;
-      __hip_atomic_store(mine + d, o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (d == 0) {
-        __hip_atomic_store(mine + D, mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(mine + D + 1, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+      put(part + (long)c * nh * (D / 2) + i, o0, o1);
+      if (d == 0) put(stats + (long)c * nh + h, mx, l);
     }
   }
   if (nsplit == 1) return;
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (tid == 0) ticket_s = __hip_atomic_fetch_add(p.tickets + pair, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (ticket_s != (unsigned)(nsplit - 1)) return;
-  for (int i = tid; i < nh * D; i += 64 * WAVES) {
-    const int h = i / D, d = i % D;
-    float gm = -INFINITY, l = 0.f, o = 0.f;
-    for (int s0 = 0; s0 < nsplit; s0 += 8) {               // eight chunks' loads in flight together
-      float pm[8], pl[8], po[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float* ps = part + ((long)min(s0 + u, nsplit - 1) * nh + h) * PW;
-        pm[u] = __hip_atomic_load(ps + D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        pl[u] = __hip_atomic_load(ps + D + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        po[u] = __hip_atomic_load(ps + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (s0 + u < nsplit) {
-          const float nm = fmaxf(gm, pm[u]);
-          const float a = __builtin_amdgcn_exp2f(gm - nm), w = __builtin_amdgcn_exp2f(pm[u] - nm);
-          l = l * a + pl[u] * w;
-          o = o * a + po[u] * w;
-          gm = nm;
-        }
+
+  // whether this workgroup is the last of `count` to come here
+  auto last_of = [&](unsigned* ticket, int count) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+      ticket_s = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (ticket_s == (unsigned)(count - 1)) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
     }
-    orow[i] = (bf16)(o / l * vscale);
+    __syncthreads();
+    return ticket_s == (unsigned)(count - 1);
+  };
+  // the partials first, first + step, ... of at most JOIN chunks, all loads in flight together: to the output, or in the first's place
+  __shared__ float2 stats_s[JOIN][16];
+  auto join = [&](int first, int step, int count, bool output) {
+    for (int i = tid; i < count * nh; i += 64 * WAVES) {
+      const unsigned long long v = get(stats + (long)(first + i / nh * step) * nh + i % nh);
+      stats_s[i / nh][i % nh] = float2{low(v), high(v)};
+    }
+    __syncthreads();
+    for (int i = tid; i < nh * D / 2; i += 64 * WAVES) {
+      const int h = i / (D / 2);
+      unsigned long long v[JOIN];
+#pragma unroll
+      for (int u = 0; u < JOIN; ++u)
+        if (u < count) v[u] = get(part + (long)(first + u * step) * nh * (D / 2) + i);
+      float mx = stats_s[0][h].x, o0 = 0.f, o1 = 0.f, l = 0.f;
+      for (int u = 1; u < count; ++u) mx = fmaxf(mx, stats_s[u][h].x);
+#pragma unroll
+      for (int u = 0; u < JOIN; ++u)
+        if (u < count) {
+          const float f = __builtin_amdgcn_exp2f(stats_s[u][h].x - mx);
+          l += stats_s[u][h].y * f;
+          o0 += low(v[u]) * f;
+          o1 += high(v[u]) * f;
+        }
+      if (output) {
+        finish(i, o0, o1, l);
+      } else {
+        put(part + (long)first * nh * (D / 2) + i, o0, o1);
+        if (i % (D / 2) == 0) put(stats + (long)first * nh + h, mx, l);
+      }
+    }
+  };
+  unsigned* tickets = p.tickets + pair * TICKETS;
+  if (nsplit <= JOIN) {
+    if (last_of(tickets, nsplit)) join(0, 1, nsplit, true);
+    return;
   }
-  if (tid == 0) __hip_atomic_store(p.tickets + pair, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // ready for the next launch
+  // groups of chunks first, then the groups
+  const int group = c / JOIN, groups = (nsplit + JOIN - 1) / JOIN, mine = min(JOIN, nsplit - group * JOIN);
+  if (!last_of(tickets + 1 + group, mine)) return;
+  join(group * JOIN, 1, mine, false);
+  if (last_of(tickets, groups)) join(0, JOIN, groups, true);
 }
 
 // What both entry points ask of a cache; 0 when it is sound.
@@ -522,13 +567,28 @@ Pool pool_of(void* base, long page, long slot, long head, const void* scale, int
 Pool k_pool(const bagel_paged_cache* c) { return pool_of(c->k, c->k_page_stride, c->k_slot_stride, c->k_head_stride, c->k_scale, c->e4m3); }
 Pool v_pool(const bagel_paged_cache* c) { return pool_of(c->v, c->v_page_stride, c->v_slot_stride, c->v_head_stride, c->v_scale, c->e4m3); }
 
-// Chunks a row is split into when no row has more than max_kv_len keys.
-int attend_splits(long rows, int Hq, int Hkv, long max_kv_len) {
-  const long pairs = rows * Hkv * ((Hq / Hkv + 15) / 16);
-  const long want = (2L * bagel_cu_count() + pairs - 1) / pairs;     // two workgroups per CU
-  return (int)std::max<long>(1, std::min<long>(std::min<long>(want, MAX_SPLITS), max_kv_len / 256));
+// Chunks that rows are split into where none has more than max_kv_len keys: whole rounds of the waves' tiles, two workgroups
+// per CU.
+struct Split {
+  int splits, chunk;
+};
+long head_blocks(int Hq, int Hkv) { return Hkv * (long)((Hq / Hkv + 15) / 16); }
+long attend_round(int D, int e4m3) { return WAVES * 32 * (D * (e4m3 ? 1 : 2) == 256 ? 1 : 2); }
+Split attend_split(long rows, int Hq, int Hkv, int D, int e4m3, long max_kv_len) {
+  const long want = std::max(1L, std::min<long>(MAX_SPLITS, 2L * bagel_cu_count() / (rows * head_blocks(Hq, Hkv))));
+  const long round = attend_round(D, e4m3), rounds = std::max(1L, (max_kv_len + round - 1) / round);
+  const long chunk = (rounds + want - 1) / want * round;
+  return Split{(int)std::max(1L, (max_kv_len + chunk - 1) / chunk), (int)chunk};
 }
-long ticket_bytes(long rows, int Hq, int Hkv) { return (rows * Hkv * ((Hq / Hkv + 15) / 16) * 4 + 255) / 256 * 256; }
+// Only rows that are split take tickets, and then there are no more (row, kv head, head block) triples than CUs: the place of
+// the tickets does not depend on the call, so that one workspace serves batches of every size.
+long ticket_bytes() { return (long)bagel_cu_count() * TICKETS * 4; }
+// Partials of the largest call with up to these rows and keys.
+long most_partials(long rows, int Hq, int Hkv, int D, int e4m3, long max_kv_len) {
+  const long round = attend_round(D, e4m3), rounds = std::max(1L, (max_kv_len + round - 1) / round);
+  const long splits = std::min<long>(MAX_SPLITS, rounds);
+  return splits > 1 ? std::min(rows * splits, 2L * bagel_cu_count() / head_blocks(Hq, Hkv)) * Hq : 0;
+}
 
 }  // namespace
 
@@ -562,8 +622,8 @@ extern "C" int bagel_paged_kv_append_bf16(const void* qkv, long ld, int rows, in
 
 extern "C" long bagel_paged_decode_attention_workspace_bytes(int rows, int Hq, int Hkv, int head_dim, long max_kv_len) {
   if (rows <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0 || max_kv_len < 0) return 0;
-  const long splits = attend_splits(rows, Hq, Hkv, max_kv_len);
-  return ticket_bytes(rows, Hq, Hkv) + (splits > 1 ? (long)rows * Hq * splits * (head_dim + 2) * 4 : 0);
+  return ticket_bytes() + std::max(most_partials(rows, Hq, Hkv, head_dim, 0, max_kv_len), most_partials(rows, Hq, Hkv, head_dim, 1, max_kv_len)) *
+                              (head_dim + 2) * 4;
 }
 
 extern "C" int bagel_paged_decode_attention_bf16(const void* Q, long ldq, int rows, int Hq, const bagel_paged_cache* cache,
@@ -587,18 +647,19 @@ extern "C" int bagel_paged_decode_attention_bf16(const void* Q, long ldq, int ro
   BAGEL_CHECK(room <= 1L << 30, "bagel_paged_decode_attention_bf16: a page table of %d pages of %d slots (at most 2^30 keys a row)",
               table_width, cache->page_size);
   const long bound = max_kv_len > 0 ? std::min(max_kv_len, room) : room;
-  const long need = bagel_paged_decode_attention_workspace_bytes(rows, Hq, Hkv, D, bound);
+  const Split split = attend_split(rows, Hq, Hkv, D, cache->e4m3, bound);
+  const long partials = split.splits > 1 ? (long)rows * Hq * split.splits : 0, need = ticket_bytes() + partials * (D + 2) * 4;
   BAGEL_CHECK(workspace_bytes >= need, "bagel_paged_decode_attention_bf16: workspace of %ld bytes, %ld needed", workspace_bytes, need);
   AttendParams p;
   p.Q = (const bf16*)Q; p.ldq = ldq; p.k = k_pool(cache); p.v = v_pool(cache);
   p.table = (const int*)page_table; p.table_stride = table_stride; p.table_width = table_width; p.num_pages = cache->num_pages;
   p.page_shift = __builtin_ctz(cache->page_size); p.kv_lens = (const int*)kv_lens; p.O = (bf16*)O; p.ldo = ldo;
-  p.tickets = (unsigned*)workspace; p.part = (float*)((char*)workspace + ticket_bytes(rows, Hq, Hkv));
+  p.tickets = (unsigned*)workspace; p.part = (float*)((char*)workspace + ticket_bytes());
   p.Hq = Hq; p.Hkv = Hkv;
-  const int splits = attend_splits(rows, Hq, Hkv, bound);
-  p.chunk = (int)((bound + splits - 1) / splits + 127) / 128 * 128;
+  p.chunk = split.chunk;
+  p.stats = (float2*)(p.part + partials * D);
   p.scale_log2 = 1.4426950408889634f * (softmax_scale != 0.f ? softmax_scale : 1.0f / sqrtf((float)D));
-  const dim3 grid(splits, Hkv * blocks, rows), block(64 * WAVES);
+  const dim3 grid(split.splits, Hkv * blocks, rows), block(64 * WAVES);
   hipStream_t st = (hipStream_t)stream;
   if (D == 128 && !cache->e4m3) hipLaunchKernelGGL((paged_attention_kernel<128, false>), grid, block, 0, st, p);
   else if (D == 128) hipLaunchKernelGGL((paged_attention_kernel<128, true>), grid, block, 0, st, p);

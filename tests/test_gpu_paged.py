@@ -439,3 +439,23 @@ def test_attention_captured_and_on_another_stream():
                 p = torch.softmax(x[r, mine] @ k64[r, :n, h].t() * d ** -0.5, -1)
                 want, mag = p @ v64[r, :n, h], p @ v64[r, :n, h].abs()
                 assert bool(((o[r, mine].double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 * 1.01 + 2.0 ** -12) * mag).all()), (t, r)
+
+
+def test_attention_workspace_serves_smaller_calls():
+    """One workspace, sized for the largest call, under batches and bounds of every size: its tickets stay where they are."""
+    K = _K()
+    ws = torch.zeros(K.paged_decode_attention_workspace_bytes(300, 14, 2, 64, 6000), device=DEV, dtype=torch.uint8)
+    for seed, lens in enumerate(([6000], [10] * 300, [700] * 64, [5999, 1], [40] * 200 + [3000] * 20, [2500] * 7, [6000], [300] * 300)):
+        c = _Case(lens, 14, 2, 64, 64, BF16, "slots first", seed=20 + seed)
+        c.run(ws=ws)
+        c.check()
+
+
+@pytest.mark.parametrize("n,rows,hq,hkv,d,dtype", [(33000, 1, 4, 1, 128, BF16), (4500, 2, 32, 1, 64, F8), (20000, 3, 17, 1, 64, BF16)])
+def test_attention_joins_in_groups(n, rows, hq, hkv, d, dtype):
+    """More chunks than are joined at once, up to all that a row may have, for one and for two blocks of heads."""
+    c = _Case([n - 777 * i for i in range(rows)], hq, hkv, d, 32, dtype, "slots first", seed=n)
+    ws = c.workspace(n)
+    first = c.run(ws=ws).clone()
+    c.check()
+    assert torch.equal(c.run(ws=ws), first) and not bool(ws[:16384].any())
