@@ -457,7 +457,7 @@ def paged_kv_append(qkv, Hq, cache: PagedCache, row_slot, Q=None, q_norm=None, k
                     eps=1e-6, und_rounding=False):
     """q/k norm + RoPE of qkv's rows; keys and values to the cache's slots ``row_slot`` (negative: padding, left alone), the
     queries to ``Q`` [rows, Hq, head_dim] (bagel_paged_kv_append_bf16).  No norm weight: no norm; no tables: no rotation."""
-    rows, D = len(qkv), cache.head_dim
+    rows, D = qkv.size(0), cache.head_dim
     if Hq < 0 or (Hq == 0 and Q is not None):
         raise RuntimeError(f"paged_kv_append: Q without query heads (Hq={Hq})")
     width = (Hq + 2 * cache.heads) * D
@@ -467,12 +467,12 @@ def paged_kv_append(qkv, Hq, cache: PagedCache, row_slot, Q=None, q_norm=None, k
         ld = _check_rows(qkv, width, "paged_kv_append: qkv")
     dev = torch.cuda.current_device() if qkv.is_cuda else -2
     here = qkv.get_device() == dev == cache.device_index == row_slot.get_device()
-    if row_slot.dtype is not torch.int32 or row_slot.dim() != 1 or len(row_slot) != rows or not row_slot.is_contiguous():
+    if row_slot.dtype is not torch.int32 or row_slot.dim() != 1 or row_slot.numel() != rows or not row_slot.is_contiguous():
         _wrong_values(row_slot, torch.int32, (rows,), "paged_kv_append: row_slot")
     q_addr = ldq = 0
     if Q is not None:
-        if len(Q) != rows:
-            raise RuntimeError(f"paged_kv_append: Q has {len(Q)} rows, qkv {rows}")
+        if Q.size(0) != rows:
+            raise RuntimeError(f"paged_kv_append: Q has {Q.size(0)} rows, qkv {rows}")
         if Q.dtype is BF16 and Q.dim() == 3 and Q.size(1) == Hq and Q.size(2) == D and Q.is_contiguous():
             ldq = Hq * D
         else:
@@ -482,17 +482,17 @@ def paged_kv_append(qkv, Hq, cache: PagedCache, row_slot, Q=None, q_norm=None, k
     norms = [0, 0]
     for i, w in enumerate((q_norm, k_norm)):
         if w is not None:
-            if w.dtype is not BF16 or w.dim() != 1 or len(w) != D or not w.is_contiguous():
+            if w.dtype is not BF16 or w.dim() != 1 or w.numel() != D or not w.is_contiguous():
                 _wrong_values(w, BF16, (D,), "paged_kv_append: norm weights")
             here = here and w.get_device() == dev
             norms[i] = w.data_ptr()
     cos_addr = sin_addr = cs_addr = table_rows = 0
     if cos_t is not None and sin_t is not None and row_cs is not None:
-        table_rows = len(cos_t)
+        table_rows = cos_t.size(0)
         for t in (cos_t, sin_t):
-            if t.dtype is not BF16 or t.dim() != 2 or t.size(1) != D or len(t) != table_rows or not t.is_contiguous():
+            if t.dtype is not BF16 or t.dim() != 2 or t.size(1) != D or t.size(0) != table_rows or not t.is_contiguous():
                 _wrong_values(t, BF16, (table_rows, D), "paged_kv_append: rotation tables")
-        if row_cs.dtype is not torch.int32 or row_cs.dim() != 1 or len(row_cs) != rows or not row_cs.is_contiguous():
+        if row_cs.dtype is not torch.int32 or row_cs.dim() != 1 or row_cs.numel() != rows or not row_cs.is_contiguous():
             _wrong_values(row_cs, torch.int32, (rows,), "paged_kv_append: row_cs")
         here = here and cos_t.get_device() == sin_t.get_device() == row_cs.get_device() == dev
         cos_addr, sin_addr, cs_addr = cos_t.data_ptr(), sin_t.data_ptr(), row_cs.data_ptr()
@@ -520,14 +520,14 @@ def paged_decode_attention(Q, cache: PagedCache, page_table, kv_lens, O, workspa
     if Q.dim() != 3 or Q.shape != O.shape or Q.size(2) != D or Q.size(1) == 0 or Q.size(1) % cache.heads:
         raise RuntimeError(f"paged_decode_attention: Q {tuple(Q.shape)} and O {tuple(O.shape)} must be [rows, a multiple of "
                            f"{cache.heads} heads, {D}]")
-    rows, Hq = len(Q), Q.size(1)
+    rows, Hq = Q.size(0), Q.size(1)
     ldq = Hq * D if Q.dtype is BF16 and Q.is_contiguous() else _check_rows(Q, Hq * D, "paged_decode_attention: Q")
     ldo = Hq * D if O.dtype is BF16 and O.is_contiguous() else _check_rows(O, Hq * D, "paged_decode_attention: O")
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or len(page_table) != rows or page_table.size(1) == 0 or \
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.size(0) != rows or page_table.size(1) == 0 or \
             page_table.stride(1) != 1:
         raise RuntimeError(f"paged_decode_attention: page_table must be int32 [{rows}, pages] with contiguous rows, got "
                            f"{page_table.dtype} {list(page_table.shape)}")
-    if kv_lens.dtype is not torch.int32 or kv_lens.dim() != 1 or len(kv_lens) != rows or not kv_lens.is_contiguous():
+    if kv_lens.dtype is not torch.int32 or kv_lens.dim() != 1 or kv_lens.numel() != rows or not kv_lens.is_contiguous():
         _wrong_values(kv_lens, torch.int32, (rows,), "paged_decode_attention: kv_lens")
     if max_kv_len < 0:
         raise RuntimeError(f"paged_decode_attention: max_kv_len {max_kv_len}")
@@ -570,7 +570,7 @@ def sample_rows(logits, uniforms, tokens, workspace, temperature=None, top_k=Non
         if t is None:
             addr.append(0)
             continue
-        if t.dtype is not dtype or t.dim() != 1 or len(t) != rows or not t.is_contiguous():
+        if t.dtype is not dtype or t.dim() != 1 or t.numel() != rows or not t.is_contiguous():
             _wrong_values(t, dtype, (rows,), "sample_rows: " + name)
         here = here and t.get_device() == dev
         addr.append(t.data_ptr())

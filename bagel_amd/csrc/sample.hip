@@ -496,7 +496,7 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
   __shared__ u64 work[CAP];                  // the tokens being sorted, or the histogram of a narrowing step
   const double* table = powers.at;
   __shared__ Sums per_wave[THREADS / 64];
-  __shared__ int first[MAX_SLICES + 1];      // where each slice's list begins when they are put together
+  __shared__ int listed_s[MAX_SLICES];       // tokens in a slice's list
   __shared__ int down[MAX_SLICES];           // a slice's first bin, counted from the row's
   __shared__ int found, lowest_cut, enough;
   __shared__ unsigned gathered;
@@ -505,6 +505,15 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
   u64* sub_mass = work;                      // [SUB]
   unsigned* sub_count = (unsigned*)(work + SUB);
 
+  // What other workgroups just wrote is two microseconds away, so the lists are on their way before anything is known of
+  // them: half the workgroup per slice, the first ten slices at once.
+  static_assert(2 * LIST == THREADS, "a thread per token of two lists");
+  constexpr int AHEAD = 5;
+  const int half = tid / LIST;
+  const u64* list = p.list + (long)row * p.slices * LIST + tid % LIST;
+  u64 ahead[AHEAD];
+#pragma unroll
+  for (int c = 0; c < AHEAD; ++c) ahead[c] = half + 2 * c < p.slices ? list[(long)(half + 2 * c) * LIST] : 0;
   Slice mine{~0ull, 0, BINS - 1};
   if (tid < p.slices) mine = p.slice[(long)row * p.slices + tid];
   const float t = row_temperature(p, row), top_p = p.top_p ? p.top_p[row] : 1.0f, min_p = p.min_p ? p.min_p[row] : 0.f, u = p.uniforms[row];
@@ -544,42 +553,22 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
     down[tid] = off;
     if (off < BINS && mine.cut < BINS - 1) atomicMin(&lowest_cut, mine.cut + off);
     if (mine.listed < k && mine.cut < BINS - 1) enough = 0;       // tokens of the top k may be missing
-    // this slice's place in the lists put together: a scan over two waves
-    int n = mine.listed;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int m = __shfl_up(n, o);
-      if ((tid & 63) >= o) n += m;
-    }
-    first[tid + 1] = n;
+    listed_s[tid] = mine.listed;
   }
-  static_assert(MAX_SLICES == 128, "two waves");
-  if (tid == 0) first[0] = 0;
   __syncthreads();
-  const int half = first[64];
-  __syncthreads();
-  if (tid >= 64 && tid < MAX_SLICES) first[tid + 1] += half;
-  __syncthreads();
-  const int listed = first[MAX_SLICES];
 
-  // f(key) of every listed token, four loads in flight
+  // f(key) of every listed token
   auto for_listed = [&](auto f) {
-    for (int i0 = tid; i0 < listed; i0 += 4 * THREADS) {
-      u64 key[4];
+    for (int s0 = half; s0 < p.slices; s0 += 2 * AHEAD) {
+      u64 key[AHEAD];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int i = i0 + c * THREADS;
-        int low = 0, high = p.slices;                  // the last slice that begins at or before i
-        while (high - low > 1) {
-          const int mid = (low + high) / 2;
-          if (first[mid] <= i) low = mid;
-          else high = mid;
-        }
-        key[c] = i < listed ? p.list[((long)row * p.slices + low) * LIST + i - first[low]] : 0;
+      for (int c = 0; c < AHEAD; ++c) {
+        key[c] = ahead[c];
+        if (s0 != half && s0 + 2 * c < p.slices) key[c] = list[(long)(s0 + 2 * c) * LIST];
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (i0 + c * THREADS < listed) f(key[c]);
+      for (int c = 0; c < AHEAD; ++c)
+        if (s0 + 2 * c < p.slices && tid % LIST < listed_s[s0 + 2 * c]) f(key[c]);
     }
   };
   auto put = [&](u64 key) {
@@ -751,19 +740,32 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
     __syncthreads();
     for (int b = tid; b < BINS; b += THREADS) mass[b] = scaled(mass[b], b, table);
   } else {
-    for (int b = tid; b < BINS; b += THREADS) {
-      u64 m = 0;
-      unsigned c = 0;
-#pragma unroll 4
-      for (int i = 0; i < p.slices; ++i) {
-        const int theirs = b - down[i];
-        const u64 both = theirs >= 0 ? p.bins[((long)row * p.slices + i) * BINS + theirs] : 0;
-        m += both & ((1ull << COUNT_SHIFT) - 1);
-        c += (unsigned)(both >> COUNT_SHIFT);
+    constexpr int N = (BINS + THREADS - 1) / THREADS;
+    u64 m[N] = {};
+    unsigned c[N] = {};
+    constexpr int B = 2 * AHEAD;
+    for (int s0 = 0; s0 < p.slices; s0 += B) {         // twenty loads in flight
+      u64 both[B][N];
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        const int sl = min(s0 + i, p.slices - 1), off = s0 + i < p.slices ? down[sl] : BINS;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const int theirs = tid + e * THREADS - off;
+          both[i][e] = theirs >= 0 && theirs < BINS ? p.bins[((long)row * p.slices + sl) * BINS + theirs] : 0;
+        }
       }
-      mass[b] = scaled(m, b, table);
-      count[b] = c;
+#pragma unroll
+      for (int i = 0; i < B; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          m[e] += both[i][e] & ((1ull << COUNT_SHIFT) - 1);
+          c[e] += (unsigned)(both[i][e] >> COUNT_SHIFT);
+        }
     }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (tid + e * THREADS < BINS) mass[tid + e * THREADS] = scaled(m[e], tid + e * THREADS, table), count[tid + e * THREADS] = c[e];
   }
   prefix<BINS>(mass, count, per_wave);
   const u64 total = mass[BINS - 1];
