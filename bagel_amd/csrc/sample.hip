@@ -86,11 +86,12 @@ struct Scale {
   double base;       // bin of the maximum
 };
 constexpr double LN2 = 0.69314718055994530942;
-__device__ __forceinline__ Scale make_scale(float top, float t) {
+__device__ __forceinline__ double per_unit(float t) { return OCTAVE / LN2 / (double)t; }
+__device__ __forceinline__ Scale make_scale(float top, float t, double per) {
 #pragma clang fp contract(off)
-  const double per = OCTAVE / LN2 / (double)t;
   return Scale{top, per, (double)t * (LN2 / OCTAVE), __builtin_floor((double)top * per)};
 }
+__device__ __forceinline__ Scale make_scale(float top, float t) { return make_scale(top, t, per_unit(t)); }
 // Token x's bin, BINS for one that weighs nothing, and `part` = v - floor(v).  The maximum is in bin 0 even where v is no
 // number (an infinite maximum, an infinite T).
 __device__ __forceinline__ int bin_of(float x, const Scale& s, double& part) {
@@ -366,6 +367,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
   __shared__ Sums per_wave[THREADS / 64];
   __shared__ float top_s[THREADS / 64];
   __shared__ int first, reach, fits;
+  __shared__ unsigned listed;
   const T* x = (const T*)p.logits + (long)row * p.ld;
   const int from = slice * C * CHUNK + 8 * tid;
   Raw<T> v[C];
@@ -379,8 +381,9 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
   const float t = row_temperature(p, row);
   const int k = row_top_k(p, row);
   const bool few = k >= 1 && k <= FEW;
+  const double per = per_unit(t);                      // while the logits are on their way
   for (int b = tid; b < BINS; b += THREADS) bins[b] = 0;
-  if (tid == 0) first = 0x7fffffff, reach = BINS - 1, fits = -1;
+  if (tid == 0) first = 0x7fffffff, reach = BINS - 1, fits = -1, listed = 0;
   float top = -INFINITY;
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -409,7 +412,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
     if (tid == 0) *out = Slice{order_key(top, first), 0, BINS - 1};
     return;
   }
-  const Scale s = make_scale(top, t);
+  const Scale s = make_scale(top, t, per);
   constexpr u64 ONE = 1ull << COUNT_SHIFT;
   static_assert(C * CHUNK <= 1 << 15, "a slice's sums fit their half of the word");
   const float low = before(edge_of(BINS - 1, s));
@@ -459,9 +462,8 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
     }
   __syncthreads();
   const int cut = min(fits, reach);
-  unsigned listed = 0;
   if (cut >= 0) {
-    // places in the list by a scan over the threads' numbers of tokens: no atomics
+    // places in the list by a scan over the lanes' numbers of tokens and one atomic per wave
     const float edge = edge_of(cut, s);
     settle();
     unsigned mine = 0;
@@ -469,18 +471,20 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int e = 0; e < 8; ++e) mine += v[c].raw(e) >= edge ? 1 : 0;
-    const unsigned upto = (unsigned)scan((u64)mine, &per_wave->mass, sizeof(Sums) / 8);
-    u64* at = p.list + ((long)row * p.slices + slice) * LIST + (upto - mine);
+    const unsigned upto = wave_scan(mine, Move32{});
+    unsigned place = 0;
+    if ((tid & 63) == 63 && upto) place = atomicAdd(&listed, upto);
+    place = __builtin_amdgcn_readlane(place, 63) + upto - mine;
+    u64* at = p.list + ((long)row * p.slices + slice) * LIST + place;
     settle();
-    if (mine && upto <= LIST)                          // always: cut is a bin that fits
+    if (mine && place + mine <= LIST)                  // always: cut is a bin that fits
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (v[c].raw(e) >= edge) *at++ = order_key(v[c].raw(e), from + c * CHUNK + e);
-    listed = min(upto, (unsigned)LIST);                                     // of the last thread: all of them, bins[cut] >> COUNT_SHIFT
   }
-  if (tid == THREADS - 1) *out = Slice{order_key(top, 0), (int)listed, cut};
+  if (tid == 0) *out = Slice{order_key(top, 0), cut < 0 ? 0 : (int)(bins[cut] >> COUNT_SHIFT), cut};
 }
 
 // ---- second launch: one workgroup per row finds the token
@@ -884,15 +888,15 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
   if (tid == 0) answer(h.key, kept);
 }
 
-// Chunks per slice: what gives the busiest CU the least to do, where a slice costs its chunks and about half a chunk's time
-// for its histogram and scans.
+// Chunks per slice: two workgroups share a CU, and one takes about 5 us + 1.6 us a chunk (2 chunks 8.3 us); whole rounds of
+// all CUs count.
 int chunks_of(int rows, int n, int f32) {
   const int most = f32 ? 2 : 4;        // 16 registers of logits: with twice as many, two workgroups no longer fit a CU
   int best = most;
   long least = 0;
   for (int c = most; c >= 1; c /= 2) {
-    const long slices = (long)rows * ((n + c * CHUNK - 1) / (c * CHUNK)), per_cu = (slices + bagel_cu_count() - 1) / bagel_cu_count();
-    if (c == most || per_cu * (2 * c + 1) < least) best = c, least = per_cu * (2 * c + 1);
+    const long slices = (long)rows * ((n + c * CHUNK - 1) / (c * CHUNK)), rounds = (slices + 2 * bagel_cu_count() - 1) / (2 * bagel_cu_count());
+    if (c == most || rounds * (3 + c) < least) best = c, least = rounds * (3 + c);
   }
   return best;
 }
