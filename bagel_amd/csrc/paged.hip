@@ -503,27 +503,34 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
       stats_s[i / nh][i % nh] = float2{low(v), high(v)};
     }
     __syncthreads();
-    for (int i = tid; i < nh * D / 2; i += 64 * WAVES) {
-      const int h = i / (D / 2);
-      unsigned long long v[JOIN];
+    // two columns per thread at a time: 32 loads in flight
+    for (int i0 = tid; i0 < nh * D / 2; i0 += 128 * WAVES) {
+      unsigned long long v[2][JOIN];
 #pragma unroll
-      for (int u = 0; u < JOIN; ++u)
-        if (u < count) v[u] = get(part + (long)(first + u * step) * nh * (D / 2) + i);
-      float mx = stats_s[0][h].x, o0 = 0.f, o1 = 0.f, l = 0.f;
-      for (int u = 1; u < count; ++u) mx = fmaxf(mx, stats_s[u][h].x);
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int u = 0; u < JOIN; ++u)
-        if (u < count) {
-          const float f = __builtin_amdgcn_exp2f(stats_s[u][h].x - mx);
-          l += stats_s[u][h].y * f;
-          o0 += low(v[u]) * f;
-          o1 += high(v[u]) * f;
+        for (int u = 0; u < JOIN; ++u)
+          if (u < count && i0 + 64 * WAVES * e < nh * D / 2) v[e][u] = get(part + (long)(first + u * step) * nh * (D / 2) + i0 + 64 * WAVES * e);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = i0 + 64 * WAVES * e, h = i / (D / 2);
+        if (i >= nh * D / 2) break;
+        float mx = stats_s[0][h].x, o0 = 0.f, o1 = 0.f, l = 0.f;
+        for (int u = 1; u < count; ++u) mx = fmaxf(mx, stats_s[u][h].x);
+#pragma unroll
+        for (int u = 0; u < JOIN; ++u)
+          if (u < count) {
+            const float f = __builtin_amdgcn_exp2f(stats_s[u][h].x - mx);
+            l += stats_s[u][h].y * f;
+            o0 += low(v[e][u]) * f;
+            o1 += high(v[e][u]) * f;
+          }
+        if (output) {
+          finish(i, o0, o1, l);
+        } else {
+          put(part + (long)first * nh * (D / 2) + i, o0, o1);
+          if (i % (D / 2) == 0) put(stats + (long)first * nh + h, mx, l);
         }
-      if (output) {
-        finish(i, o0, o1, l);
-      } else {
-        put(part + (long)first * nh * (D / 2) + i, o0, o1);
-        if (i % (D / 2) == 0) put(stats + (long)first * nh + h, mx, l);
       }
     }
   };
