@@ -43,7 +43,8 @@ constexpr int LIST = 512;            // tokens that a slice lists at most
 constexpr int FEW = 512;             // a top-k up to here is looked for in the lists first
 constexpr int THREADS = 1024;
 constexpr int CHUNK = 8 * THREADS;   // logits that a workgroup loads at a time
-constexpr int MAX_SLICES = 128;      // 2^20 logits in single chunks
+constexpr int MAX_SLICES = 128;
+constexpr int MAX_TOKENS = 1 << 20;
 
 struct Slice {       // what the first launch says of a slice
   u64 best;          // the order key of its first maximum (where it is not greedy: of the maximum and no index)
@@ -54,7 +55,6 @@ struct Params {
   const void* logits;
   long ld;
   int n, slices;
-  bool vec;                          // rows start on 16-byte boundaries
   const float *uniforms, *temperature, *top_p, *min_p;
   const int* top_k;
   int* tokens;
@@ -233,29 +233,40 @@ struct Raw<float> {
   __device__ __forceinline__ void settle() { asm volatile("" : "+v"(w[0]), "+v"(w[1])); }
 };
 
-// A row's chunk of eight logits from index i on (a multiple of 8), -inf behind the row's end.
+// A row for loads of 16 bytes wherever it starts: places count from the boundary before it, `off` logits ahead of the first.
 template <typename T>
-__device__ __forceinline__ Raw<T> load_raw(const Params& p, const T* row, int i) {
-  if (p.vec && i + 8 <= p.n) return *(const Raw<T>*)(row + i);
-  T w[8];
+struct Row {
+  const T* x;        // place 0, which may be in front of the row
+  int off, end;      // the row is at the places [off, end)
+  __device__ __forceinline__ Row(const Params& p, int row) {
+    const T* first = (const T*)p.logits + (long)row * p.ld;
+    off = (int)((uintptr_t)first % 16 / sizeof(T));
+    x = first - off;
+    end = off + p.n;
+  }
+  // eight logits from place i on (a multiple of 8), -inf outside the row
+  __device__ __forceinline__ Raw<T> load(int i) const {
+    if (i >= off && i + 8 <= end) return *(const Raw<T>*)(x + i);
+    T w[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = i + e < p.n ? row[i + e] : (T)-INFINITY;
-  return __builtin_bit_cast(Raw<T>, w);
-}
+    for (int e = 0; e < 8; ++e) w[e] = i + e >= off && i + e < end ? x[i + e] : (T)-INFINITY;
+    return __builtin_bit_cast(Raw<T>, w);
+  }
+};
 // f(value, index) for this thread's share of a whole row's logits in [least, beyond) - a NaN for beyond: no upper end -, four
 // loads in flight.
 template <typename T, typename F>
 __device__ __forceinline__ void for_range(const Params& p, int row, float least, float beyond, F f) {
-  const T* x = (const T*)p.logits + (long)row * p.ld;
+  const Row<T> r(p, row);
   constexpr int N = 4;
-  for (int i0 = 8 * (int)threadIdx.x; i0 < p.n; i0 += N * CHUNK) {
+  for (int i0 = 8 * (int)threadIdx.x; i0 < r.end; i0 += N * CHUNK) {
     Raw<T> v[N];
-    if (p.vec && i0 + (N - 1) * CHUNK + 8 <= p.n) {
+    if (i0 >= r.off && i0 + (N - 1) * CHUNK + 8 <= r.end) {
 #pragma unroll
-      for (int c = 0; c < N; ++c) v[c] = *(const Raw<T>*)(x + i0 + c * CHUNK);
+      for (int c = 0; c < N; ++c) v[c] = *(const Raw<T>*)(r.x + i0 + c * CHUNK);
     } else {
 #pragma unroll
-      for (int c = 0; c < N; ++c) v[c] = load_raw(p, x, i0 + c * CHUNK);
+      for (int c = 0; c < N; ++c) v[c] = r.load(i0 + c * CHUNK);
     }
     // first which, then f: few lanes have one at the same place, and what f waits for is waited for once per round
     unsigned hits = 0;
@@ -265,7 +276,7 @@ __device__ __forceinline__ void for_range(const Params& p, int row, float least,
       for (int e = 0; e < 8; ++e) hits |= (unsigned)(v[c].raw(e) >= least && !(v[c].raw(e) >= beyond)) << (8 * c + e);
     for (; hits; hits &= hits - 1) {
       const int bit = __ffs(hits) - 1, i = i0 + bit / 8 * CHUNK + bit % 8;
-      f((float)x[i], i);
+      f((float)r.x[i], i - r.off);
     }
   }
 }
@@ -368,15 +379,15 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
   __shared__ float top_s[THREADS / 64];
   __shared__ int first, reach, fits;
   __shared__ unsigned listed;
-  const T* x = (const T*)p.logits + (long)row * p.ld;
-  const int from = slice * C * CHUNK + 8 * tid;
+  const Row<T> r(p, row);
+  const int place = slice * C * CHUNK + 8 * tid, from = place - r.off;      // in the row with what is ahead of it; in the row
   Raw<T> v[C];
-  if (p.vec && (slice + 1) * C * CHUNK <= p.n) {       // every load at once
+  if (slice * C * CHUNK >= r.off && (slice + 1) * C * CHUNK <= r.end) {       // every load at once
 #pragma unroll
-    for (int c = 0; c < C; ++c) v[c] = *(const Raw<T>*)(x + from + c * CHUNK);
+    for (int c = 0; c < C; ++c) v[c] = *(const Raw<T>*)(r.x + place + c * CHUNK);
   } else {
 #pragma unroll
-    for (int c = 0; c < C; ++c) v[c] = load_raw(p, x, from + c * CHUNK);
+    for (int c = 0; c < C; ++c) v[c] = r.load(place + c * CHUNK);
   }
   const float t = row_temperature(p, row);
   const int k = row_top_k(p, row);
@@ -472,12 +483,12 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) mine += v[c].raw(e) >= edge ? 1 : 0;
     const unsigned upto = wave_scan(mine, Move32{});
-    unsigned place = 0;
-    if ((tid & 63) == 63 && upto) place = atomicAdd(&listed, upto);
-    place = __builtin_amdgcn_readlane(place, 63) + upto - mine;
-    u64* at = p.list + ((long)row * p.slices + slice) * LIST + place;
+    unsigned base = 0;
+    if ((tid & 63) == 63 && upto) base = atomicAdd(&listed, upto);
+    base = __builtin_amdgcn_readlane(base, 63) + upto - mine;
+    u64* at = p.list + ((long)row * p.slices + slice) * LIST + base;
     settle();
-    if (mine && place + mine <= LIST)                  // always: cut is a bin that fits
+    if (mine && base + mine <= LIST)                  // always: cut is a bin that fits
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -890,44 +901,50 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
 
 // Chunks per slice: two workgroups share a CU, and one takes about 5 us + 1.6 us a chunk (2 chunks 8.3 us); whole rounds of
 // all CUs count.
+int slices_of(int n, int chunks) { return (n + chunks * CHUNK - 1) / (chunks * CHUNK); }
 int chunks_of(int rows, int n, int f32) {
   const int most = f32 ? 2 : 4;        // 16 registers of logits: with twice as many, two workgroups no longer fit a CU
   int best = most;
   long least = 0;
-  for (int c = most; c >= 1; c /= 2) {
-    const long slices = (long)rows * ((n + c * CHUNK - 1) / (c * CHUNK)), rounds = (slices + 2 * bagel_cu_count() - 1) / (2 * bagel_cu_count());
+  for (int c = most; c >= 1 && slices_of(n, c) <= MAX_SLICES; c /= 2) {
+    const long rounds = ((long)rows * slices_of(n, c) + 2 * bagel_cu_count() - 1) / (2 * bagel_cu_count());
     if (c == most || rounds * (3 + c) < least) best = c, least = rounds * (3 + c);
   }
   return best;
 }
-int slices_of(int n, int chunks) { return (n + chunks * CHUNK - 1) / (chunks * CHUNK); }
-long workspace_of(int rows, int n, int f32) { return (long)rows * slices_of(n, chunks_of(rows, n, f32)) * (sizeof(Slice) + LIST * 8 + BINS * 8); }
+// Rows that do not start on 16-byte boundaries reach up to seven places further.
+int places_of(int n) { return n + 7; }
+long workspace_of(int rows, int n, int f32) {
+  return (long)rows * slices_of(places_of(n), chunks_of(rows, places_of(n), f32)) * (sizeof(Slice) + LIST * 8 + BINS * 8);
+}
 
 }  // namespace
 
 extern "C" long bagel_sample_rows_workspace_bytes(int rows, int n) {
-  return rows <= 0 || n <= 0 ? 0 : std::max(workspace_of(rows, n, 0), workspace_of(rows, n, 1));
+  long most = 0;       // fewer rows can be cut into more slices altogether
+  if (n > 0 && n <= MAX_TOKENS)
+    for (int r = 1; r <= rows; ++r) most = std::max(most, std::max(workspace_of(r, n, 0), workspace_of(r, n, 1)));
+  return most;
 }
 
 extern "C" int bagel_sample_rows(const void* logits, long ld, int rows, int n, int logits_f32, const void* uniforms, const void* temperature,
                                  const void* top_k, const void* top_p, const void* min_p, void* tokens, void* logprobs,
                                  void* workspace, long workspace_bytes, void* stream) {
   BAGEL_CHECK(rows >= 0 && rows <= 65535, "bagel_sample_rows: rows=%d (at most 65535)", rows);
-  BAGEL_CHECK(n > 0 && n <= MAX_SLICES * CHUNK, "bagel_sample_rows: %d tokens (1 to 2^20)", n);
+  BAGEL_CHECK(n > 0 && n <= MAX_TOKENS, "bagel_sample_rows: %d tokens (1 to 2^20)", n);
   BAGEL_CHECK(logits_f32 == 0 || logits_f32 == 1, "bagel_sample_rows: logits_f32=%d", logits_f32);
   if (rows == 0) return 0;
   BAGEL_CHECK(logits && uniforms && tokens && workspace, "bagel_sample_rows: null operand");
   BAGEL_CHECK(ld >= n || ld == 0, "bagel_sample_rows: leading dim %ld below %d tokens", ld, n);
   BAGEL_CHECK((uintptr_t)logits % (logits_f32 ? 4 : 2) == 0 && (uintptr_t)workspace % 16 == 0, "bagel_sample_rows: misaligned operand");
-  BAGEL_CHECK(workspace_bytes >= bagel_sample_rows_workspace_bytes(rows, n), "bagel_sample_rows: workspace of %ld bytes, %ld needed",
-              workspace_bytes, bagel_sample_rows_workspace_bytes(rows, n));
+  const long need = workspace_of(rows, n, logits_f32);
+  BAGEL_CHECK(workspace_bytes >= need, "bagel_sample_rows: workspace of %ld bytes, %ld needed", workspace_bytes, need);
   Params p;
   p.logits = logits; p.ld = ld; p.n = n;
-  p.vec = (uintptr_t)logits % 16 == 0 && ld % (logits_f32 ? 4 : 8) == 0;
   p.uniforms = (const float*)uniforms; p.temperature = (const float*)temperature; p.top_k = (const int*)top_k;
   p.top_p = (const float*)top_p; p.min_p = (const float*)min_p; p.tokens = (int*)tokens; p.logprobs = (float*)logprobs;
-  const int c = chunks_of(rows, n, logits_f32);
-  p.slices = slices_of(n, c);
+  const int c = chunks_of(rows, places_of(n), logits_f32);
+  p.slices = slices_of(places_of(n), c);
   const long slices = (long)rows * p.slices;
   p.slice = (Slice*)workspace;
   p.list = (u64*)(p.slice + slices);

@@ -170,6 +170,44 @@ def test_sampling_strides(dtype):
     _check(wide[4:5, 3:77].expand(50, -1), **_settings(50, gen, n=74))
 
 
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_sampling_of_rows_at_every_address(dtype):
+    """A vocabulary of odd size puts its rows on every boundary; so do views that begin inside a row."""
+    gen = torch.Generator(device=DEV).manual_seed(17)
+    for n in (1, 3, 9, 8191, 8193, 16385, 33333):
+        _check(_logits(9, n, gen, dtype), **_settings(9, gen, n=n), what=n)
+        _check(_logits(9, n, gen, dtype), **_settings(9, gen, n=n, k=0, p=1.0, m=0.0), what=n)
+    flat = _logits(1, 40000, gen, dtype)[0]
+    for first in range(1, 9):
+        for n in (5, 8192 - first, 8192, 20000):
+            x = flat[first:first + n][None]
+            x[0, -1] = 30.0                                  # the last one of the row, and what lies beyond it, count or not
+            _check(x, **_settings(1, gen, n=n), what=(first, n))
+    x = torch.full((6, 70001), -INF, device=DEV).to(dtype)
+    _check(x, **_settings(6, gen, t=0.0), what="nothing")
+    _check(x, **_settings(6, gen), what="nothing")
+
+
+def test_sampling_of_the_largest_row():
+    gen = torch.Generator(device=DEV).manual_seed(18)
+    n = 1 << 20
+    wide = _logits(2, n + 3, gen, BF16)
+    _check(wide[:, 1:n + 1], **_settings(2, gen, n=n))
+    _check(wide[:, :n], **_settings(2, gen, n=n, k=0, p=0.9))
+
+
+def test_sampling_workspace_serves_fewer_rows():
+    K = _K()
+    gen = torch.Generator(device=DEV).manual_seed(19)
+    n = 50001
+    ws = torch.full((K.sample_rows_workspace_bytes(70, n),), 0x77, device=DEV, dtype=torch.uint8)
+    for rows in (70, 1, 13, 64, 33):
+        x, s = _logits(rows, n, gen, BF16), _settings(rows, gen, n=n)
+        tokens = torch.empty(rows, device=DEV, dtype=torch.int32)
+        K.sample_rows(x, s["u"], tokens, ws, temperature=s["t"], top_k=s["k"], top_p=s["p"], min_p=s["m"])
+        assert torch.equal(tokens.long(), _want(x, **s)[0])
+
+
 def test_sampling_does_not_depend_on_the_batch():
     gen = torch.Generator(device=DEV).manual_seed(8)
     x = _logits(64, 152064, gen, BF16)

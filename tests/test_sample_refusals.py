@@ -45,4 +45,10 @@ def test_c_sampling_refusals(change, message):
 
 def test_no_rows_is_no_error():
     assert _c_sample(rows=0, logits=None, u=None, tokens=None, ws=None) == 0
-    assert K.sample_rows_workspace_bytes(0, 100) == 0
+    assert K.sample_rows_workspace_bytes(0, 100) == 0 and K.sample_rows_workspace_bytes(5, 0) == 0
+
+
+def test_workspace_serves_fewer_rows():
+    for n in (1000, 32000, 61265, 152064, 1 << 20):
+        sizes = [K.sample_rows_workspace_bytes(rows, n) for rows in range(1, 90)]
+        assert sizes == sorted(sizes) and sizes[0] > 0
