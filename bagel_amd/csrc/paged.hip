@@ -141,19 +141,26 @@ int launch_append(const AppendParams& p, hipStream_t st) {
 // The keys and values of a (row, kv head) are read once for all the query heads that share them, up to 16 per workgroup,
 // so that the matrix instruction's 16 columns are heads:
 //   S^T[key][head] = K . Q^T      and      O^T[d][head] += V^T . P^T
-// with 32 keys as the contraction of the second product.  Nothing passes through LDS on the way:
-//   - A lane of S^T's operand holds 16 bytes of ONE key row (lane & 15 = row, lane >> 4 = part of the contraction).
+// with 32 keys as the contraction of the second product.
+//   - Key rows go to LDS whole, without passing a register, and a lane of S^T's operand reads 16 bytes of ONE key row
+//     (lane & 15 = row, lane >> 4 = part of the contraction).
 //   - Row m of key tile t is key 8 (m / 4) + 4 t + m % 4 of the 32, so that the results a lane gets - rows 4 g + i of both
 //     tiles, g = lane >> 4 - are keys 8 g ... 8 g + 7 of its head: exactly what the second product wants of P^T from it.
-//   - V rows are read whole (16 lanes x D / 16 elements, 8 keys per lane group).  The operand wants 8 KEYS of one d per
+//   - V rows go to registers (16 lanes x D / 16 elements, 8 keys per lane group).  The operand wants 8 KEYS of one d per
 //     lane; the lane has D / 16 d's of those 8 keys, so byte permutes turn one into the other inside the lane, and
 //     row r of product dd is d = (D / 16) r + dd.
 // The softmax is the running form: one maximum and sum per head and wave, scores and sums in fp32, P rounded to bf16 for
 // the matrix product (an error of 2^-9 of each weight, which the output's own rounding to bf16 exceeds).
 // An e4m3 value is a bf16 value: keys and values are widened exactly, the scales enter in fp32.
 //
-// One workgroup = four waves that take turns at the chunk's tiles, each with its own running softmax.  A row with more keys than one chunk is split over workgroups; each leaves an
-// unnormalised partial (sums in fp32) and the last one to finish joins them in chunk order.
+// One workgroup = four waves that take turns at the chunk's tiles, each with its own running softmax.  A row with more keys
+// than one chunk is split over workgroups; each leaves an unnormalised partial (sums in fp32) and the last one to finish
+// joins them in chunk order, JOIN at a time: more chunks than that are joined in groups first.
+//
+// Bound by the reads of the cache.  28 query and 4 kv heads of 128 (times with the launch): 64 rows of up to 8192 keys, 604 MB
+// of bf16, 108 us = 5.6 TB/s; one row of 131072, 268 MB, 57 us, joins included; e4m3 with 8 kv heads, 200 rows of up
+// to 4096, 475 MB, 94 us = 5.1 TB/s.  Reads of random 16 KB pages alone reach 6.9 TB/s past the caches, 6.0 through them.
+// Keys straight to registers, 16 bytes of each of 16 rows per lane: 128 us for the first and 115 for the last of these.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int WAVES = 4;
 constexpr int JOIN = 16;             // partials that are joined at once
@@ -262,8 +269,8 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
   struct Tile {
     unsigned v[SUB][8][VW];
   };
-  // Page ids of the tile at key k0, one per lane group and block of 32: that of keys 8 g ... 8 g + 7, of which no page holds a
-  // part.  A page id outside the pool is not followed: the row's output says so instead.
+  // Page ids of the tile at key k0, one per lane group and block of 32: that of keys 8 g ... 8 g + 7, which share a
+  // page.  A page id outside the pool is not followed: the row's output says so instead.
   auto load_ids = [&](int (&ids)[SUB], int k0) {
 #pragma unroll
     for (int s = 0; s < SUB; ++s) ids[s] = table[min((k0 + 32 * s + 8 * g) >> p.page_shift, last_page)];
@@ -327,7 +334,9 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
   f32x4 acc[ND];
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = -INFINITY, l_run = 0.f;        // l_run: this lane's keys only
+  // The maximum starts at the lowest number and not at -inf: scores of -inf (keys that hold infinities) weigh nothing even
+  // where a wave or a chunk has no others.
+  float m_run = -3.402823466e38f, l_run = 0.f; // l_run: this lane's keys only
 
   typedef float Scores[SUB][8];
   auto scores = [&](Scores& s) {
@@ -463,7 +472,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
   auto high = [](unsigned long long v) { return __uint_as_float((unsigned)(v >> 32)); };
   for (int i = tid; i < nh * D / 2; i += 64 * WAVES) {
     const int h = i / (D / 2), d = 2 * (i % (D / 2));
-    float mx = m_s[0][h];                                   // wave 0 always had a tile
+    float mx = m_s[0][h];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) mx = fmaxf(mx, m_s[w][h]);
     float o0 = 0.f, o1 = 0.f, l = 0.f;

@@ -923,7 +923,7 @@ long workspace_of(int rows, int n, int f32) {
 extern "C" long bagel_sample_rows_workspace_bytes(int rows, int n) {
   long most = 0;       // fewer rows can be cut into more slices altogether
   if (n > 0 && n <= MAX_TOKENS)
-    for (int r = 1; r <= rows; ++r) most = std::max(most, std::max(workspace_of(r, n, 0), workspace_of(r, n, 1)));
+    for (int r = 1; r <= std::min(rows, 65535); ++r) most = std::max(most, std::max(workspace_of(r, n, 0), workspace_of(r, n, 1)));
   return most;
 }
 

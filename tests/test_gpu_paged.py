@@ -362,6 +362,24 @@ def test_attention_nan_reaches_its_heads_only():
     assert bool(torch.isinf(out[1, :2, 7]).all()) and bool(torch.isfinite(out[1, 2:]).all()) and bool(torch.isfinite(out[1, :2, :7]).all())
 
 
+@pytest.mark.parametrize("rows,n", [(1, 2500), (1, 33000), (300, 400)])
+def test_attention_keys_of_infinite_scores(rows, n):
+    """Scores of -inf weigh nothing, where they fill a tile, a wave's share or a chunk too; a row of nothing else is 0 / 0."""
+    c = _Case([n - 17 * (i % 8) for i in range(rows)], 14, 2, 64, 16, BF16, "slots first", seed=12)
+    c.q[:, :, 0] = 1.0
+    at = torch.arange(n, device=DEV)
+    for r, length in enumerate(c.lens[:8]):
+        # from the first rows' ends backwards 1, 65, ... keys, or the first ones, or all but one in the middle
+        masked = at[:length]
+        masked = {0: masked[length // 2 + 1:], 1: masked[-1:], 2: masked[-65:], 3: masked[:-1], 4: masked[:300], 5: masked[masked != 130],
+                  6: masked, 7: masked[128:192]}[r]
+        c.kp[c.table[r].long()[masked // 16], masked % 16, :, 0] = float("-inf")
+    c.run()
+    if rows > 6:
+        assert bool(torch.isnan(c.out()[6]).all())
+    c.check(rows=[r for r in range(rows) if r != 6])
+
+
 @pytest.mark.parametrize("dtype,hkv", [(BF16, 4), (F8, 8)])
 def test_attention_and_append_past_32_bits(dtype, hkv):
     """A pool of more than 2^32 bytes: pages at its far end are written and read."""

@@ -58,7 +58,7 @@ def _check(logits, u, t, k, p, m, what=""):
     token, logprob = _want(logits, u, t, k, p, m)
     off = torch.nonzero(tokens.long() != token)[:, 0].tolist()
     assert not off, (what, [(r, int(tokens[r]), int(token[r]), float(u[r]), float(t[r]), int(k[r]), float(p[r]), float(m[r])) for r in off[:4]])
-    # one rounding to 32 bits of a 64-bit value; the weights' units move their sum by at most n / 2 of 2^-44, below 2^-25 of it
+    # one rounding to 32 bits of a 64-bit value; weights good to 2^-32 of themselves move the logarithm of their sum below 2^-31
     fine = torch.isfinite(logprob)
     assert torch.equal(fine, torch.isfinite(logprobs)), what
     assert bool(((logprobs.double() - logprob).abs()[fine] <= 2.0 ** -24 * logprob.abs()[fine] + 2.0 ** -24).all()), what
