@@ -367,7 +367,7 @@ def decode_attention(qkv, Hq, Hkv, D, q_norm, k_norm, cos_t, sin_t, row_cs, row_
 # ---- a paged key-value cache ---------------------------------------------------------------------
 # A step of a serving loop is a few microseconds on the device, so these wrappers are written for the host's time too: what
 # can be checked once is checked when a PagedCache is made, argument types are declared to ctypes instead of being wrapped
-# per call, messages are only made when something is wrong (an append with its launch: 9 us on the host; 17 us without all this).
+# per call, messages are only made when something is wrong (an append with its launch: 8 us on the host; 17 us without all this).
 E4M3 = torch.float8_e4m3fn
 BF16 = torch.bfloat16
 
@@ -448,6 +448,11 @@ def _declared(name, *types):
     return fn
 
 
+def _current_device():
+    """torch.cuda.current_device() where there is a device tensor already (nothing to initialise)."""
+    return torch._C._cuda_getDevice()
+
+
 def _raw_stream(dev):
     """The current stream of device ``dev`` (checked to be the current one) as an address."""
     return torch._C._cuda_getCurrentRawStream(dev)
@@ -457,25 +462,26 @@ def paged_kv_append(qkv, Hq, cache: PagedCache, row_slot, Q=None, q_norm=None, k
                     eps=1e-6, und_rounding=False):
     """q/k norm + RoPE of qkv's rows; keys and values to the cache's slots ``row_slot`` (negative: padding, left alone), the
     queries to ``Q`` [rows, Hq, head_dim] (bagel_paged_kv_append_bf16).  No norm weight: no norm; no tables: no rotation."""
-    rows, D = qkv.size(0), cache.head_dim
+    shape, D = qkv.shape, cache.head_dim
+    rows = shape[0]
     if Hq < 0 or (Hq == 0 and Q is not None):
         raise RuntimeError(f"paged_kv_append: Q without query heads (Hq={Hq})")
     width = (Hq + 2 * cache.heads) * D
-    if qkv.dtype is BF16 and qkv.dim() == 2 and qkv.size(1) == width and qkv.is_contiguous():
+    if qkv.dtype is BF16 and shape == (rows, width) and qkv.is_contiguous():
         ld = width
     else:
         ld = _check_rows(qkv, width, "paged_kv_append: qkv")
-    dev = torch.cuda.current_device() if qkv.is_cuda else -2
+    dev = _current_device() if qkv.is_cuda else -2
     here = qkv.get_device() == dev == cache.device_index == row_slot.get_device()
     if row_slot.dtype is not torch.int32 or row_slot.dim() != 1 or row_slot.numel() != rows or not row_slot.is_contiguous():
         _wrong_values(row_slot, torch.int32, (rows,), "paged_kv_append: row_slot")
     q_addr = ldq = 0
     if Q is not None:
-        if Q.size(0) != rows:
-            raise RuntimeError(f"paged_kv_append: Q has {Q.size(0)} rows, qkv {rows}")
-        if Q.dtype is BF16 and Q.dim() == 3 and Q.size(1) == Hq and Q.size(2) == D and Q.is_contiguous():
+        if Q.dtype is BF16 and Q.shape == (rows, Hq, D) and Q.is_contiguous():
             ldq = Hq * D
         else:
+            if Q.size(0) != rows:
+                raise RuntimeError(f"paged_kv_append: Q has {Q.size(0)} rows, qkv {rows}")
             ldq = _check_rows(Q, Hq * D, "paged_kv_append: Q")
         here = here and Q.get_device() == dev
         q_addr = Q.data_ptr()
@@ -490,7 +496,7 @@ def paged_kv_append(qkv, Hq, cache: PagedCache, row_slot, Q=None, q_norm=None, k
     if cos_t is not None and sin_t is not None and row_cs is not None:
         table_rows = cos_t.size(0)
         for t in (cos_t, sin_t):
-            if t.dtype is not BF16 or t.dim() != 2 or t.size(1) != D or t.size(0) != table_rows or not t.is_contiguous():
+            if t.dtype is not BF16 or t.shape != (table_rows, D) or not t.is_contiguous():
                 _wrong_values(t, BF16, (table_rows, D), "paged_kv_append: rotation tables")
         if row_cs.dtype is not torch.int32 or row_cs.dim() != 1 or row_cs.numel() != rows or not row_cs.is_contiguous():
             _wrong_values(row_cs, torch.int32, (rows,), "paged_kv_append: row_cs")
@@ -517,14 +523,15 @@ def paged_decode_attention(Q, cache: PagedCache, page_table, kv_lens, O, workspa
     Q, O [rows, Hq, head_dim]; page_table [rows, pages] int32; workspace: paged_decode_attention_workspace_bytes, made with
     torch.zeros; max_kv_len: an upper bound of kv_lens known on the host (0: the table's width)."""
     D = cache.head_dim
-    if Q.dim() != 3 or Q.shape != O.shape or Q.size(2) != D or Q.size(1) == 0 or Q.size(1) % cache.heads:
+    shape = Q.shape
+    if len(shape) != 3 or shape != O.shape or shape[2] != D or shape[1] == 0 or shape[1] % cache.heads:
         raise RuntimeError(f"paged_decode_attention: Q {tuple(Q.shape)} and O {tuple(O.shape)} must be [rows, a multiple of "
                            f"{cache.heads} heads, {D}]")
-    rows, Hq = Q.size(0), Q.size(1)
+    rows, Hq, _ = shape
     ldq = Hq * D if Q.dtype is BF16 and Q.is_contiguous() else _check_rows(Q, Hq * D, "paged_decode_attention: Q")
     ldo = Hq * D if O.dtype is BF16 and O.is_contiguous() else _check_rows(O, Hq * D, "paged_decode_attention: O")
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.size(0) != rows or page_table.size(1) == 0 or \
-            page_table.stride(1) != 1:
+    table = page_table.shape
+    if page_table.dtype is not torch.int32 or len(table) != 2 or table[0] != rows or table[1] == 0 or page_table.stride(1) != 1:
         raise RuntimeError(f"paged_decode_attention: page_table must be int32 [{rows}, pages] with contiguous rows, got "
                            f"{page_table.dtype} {list(page_table.shape)}")
     if kv_lens.dtype is not torch.int32 or kv_lens.dim() != 1 or kv_lens.numel() != rows or not kv_lens.is_contiguous():
@@ -535,11 +542,11 @@ def paged_decode_attention(Q, cache: PagedCache, page_table, kv_lens, O, workspa
         raise RuntimeError(f"paged_decode_attention: softmax_scale {softmax_scale}")
     if not workspace.is_contiguous():
         raise RuntimeError("paged_decode_attention: contiguous workspace expected")
-    dev = torch.cuda.current_device() if Q.is_cuda else -2
+    dev = _current_device() if Q.is_cuda else -2
     if not (Q.get_device() == dev == O.get_device() == page_table.get_device() == kv_lens.get_device() == workspace.get_device() ==
             cache.device_index):
         _not_here(Q, page_table, kv_lens, O, workspace, cache.k_pages)
-    width = page_table.size(1)
+    width = table[1]
     fn = _declared("bagel_paged_decode_attention_bf16", VP, L, I, I, VP, VP, L, I, VP, L, VP, L, F, VP, L, VP)
     rc = fn(Q.data_ptr(), ldq, rows, Hq, cache.ref, page_table.data_ptr(), page_table.stride(0) if rows > 1 else width, width,
             kv_lens.data_ptr(), max_kv_len, O.data_ptr(), ldo, softmax_scale or 0.0, workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
@@ -561,7 +568,7 @@ def sample_rows(logits, uniforms, tokens, workspace, temperature=None, top_k=Non
         raise RuntimeError(f"sample_rows: bfloat16 or float32 logits [rows, tokens] with contiguous rows expected, got {logits.dtype} "
                            f"{tuple(logits.shape)}")
     rows, n = logits.shape
-    dev = torch.cuda.current_device() if logits.is_cuda else -2
+    dev = _current_device() if logits.is_cuda else -2
     here = logits.get_device() == dev == workspace.get_device()
     addr = []
     for name, t, dtype in (("uniforms", uniforms, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
