@@ -123,7 +123,7 @@ __device__ __forceinline__ float edge_of(int b, const Scale& s) {
   const double lowest = s.base - b;
   const float x = next((float)(lowest * s.inverse), (int)(threadIdx.x & 63) - 32);
   const u64 inside = __ballot((double)x * s.per >= lowest);      // false for what lies below -inf in the bits' order: NaN
-  return __shfl(x, inside ? __ffsll(inside) - 1 : 63);
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), inside ? __ffsll(inside) - 1 : 63));
 }
 // 2^(part / 32) in steps: a cubic through its values at the four Chebyshev points of [0, 1] (7e-11 of it off at most); a sum
 // with 2^52 leaves the rounded steps in the low bits.
@@ -312,29 +312,40 @@ struct Move32 {
 };
 __device__ __forceinline__ u64 wave_scan(u64 v) { return wave_scan(v, Move64{}); }
 constexpr int WAVES = THREADS / 64;
-__device__ __forceinline__ u64 scan(u64 v, u64* per_wave, int stride) {
-  const int wave = threadIdx.x >> 6;
-  v = wave_scan(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) per_wave[wave * stride] = v;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WAVES - 1; ++w) v += w < wave ? per_wave[w * stride] : 0;
+// What the waves below hold, from the lanes' scan of the waves' totals.
+static_assert(WAVES == 16, "a lane of a row per wave");
+template <typename V, typename F>
+__device__ __forceinline__ V row_scan(V v, F moved) {
+  v += moved.template operator()<0x111, 0xf>(v);
+  v += moved.template operator()<0x112, 0xf>(v);
+  v += moved.template operator()<0x114, 0xf>(v);
+  v += moved.template operator()<0x118, 0xf>(v);
   return v;
 }
+__device__ __forceinline__ unsigned below(unsigned total) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  return wave ? __builtin_amdgcn_readlane(row_scan(total, Move32{}), wave - 1) : 0;
+}
+__device__ __forceinline__ u64 below(u64 total) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const u64 v = row_scan(total, Move64{});
+  return wave ? ((u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), wave - 1) << 32) | (unsigned)__builtin_amdgcn_readlane((int)v, wave - 1) : 0;
+}
+__device__ __forceinline__ u64 scan(u64 v, u64* per_wave, int stride) {
+  v = wave_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) per_wave[(threadIdx.x >> 6) * stride] = v;
+  __syncthreads();
+  return v + below(per_wave[(threadIdx.x & 15) * stride]);
+}
 __device__ __forceinline__ Sums scan(Sums v, Sums* per_wave) {
-  const int wave = threadIdx.x >> 6;
   v.mass = wave_scan(v.mass);
   v.count = wave_scan(v.count, Move32{});
   __syncthreads();
-  if ((threadIdx.x & 63) == 63) per_wave[wave] = v;
+  if ((threadIdx.x & 63) == 63) per_wave[threadIdx.x >> 6] = v;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WAVES - 1; ++w) {
-    v.mass += w < wave ? per_wave[w].mass : 0;
-    v.count += w < wave ? per_wave[w].count : 0;
-  }
-  return v;
+  const Sums total = per_wave[threadIdx.x & 15];
+  return Sums{v.mass + below(total.mass), v.count + below(total.count)};
 }
 // Bins -> sums up to and including them (two neighbours per thread).
 template <int N>
@@ -375,10 +386,10 @@ template <typename T, int C>
 __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
   const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
   __shared__ u64 bins[BINS];
-  __shared__ Sums per_wave[THREADS / 64];
+  __shared__ unsigned count_s[THREADS / 64];
   __shared__ float top_s[THREADS / 64];
   __shared__ int first, reach, fits;
-  __shared__ unsigned listed;
+  __shared__ unsigned listed, reach_count, fits_count;
   const Row<T> r(p, row);
   const int place = slice * C * CHUNK + 8 * tid, from = place - r.off;      // in the row with what is ahead of it; in the row
   Raw<T> v[C];
@@ -394,7 +405,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
   const bool few = k >= 1 && k <= FEW;
   const double per = per_unit(t);                      // while the logits are on their way
   for (int b = tid; b < BINS; b += THREADS) bins[b] = 0;
-  if (tid == 0) first = 0x7fffffff, reach = BINS - 1, fits = -1, listed = 0;
+  if (tid == 0) first = 0x7fffffff, reach = BINS, fits = -1, listed = 0;
   float top = -INFINITY;
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -464,13 +475,24 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
     for (int b = tid; b < BINS; b += THREADS) at[b] = bins[b];
   }
   // the list: the bins up to `cut`, the last that fits or, for a top-k of a few, the first that brings k tokens
-  prefix<BINS>(bins, per_wave);
-  for (int b = 2 * tid; b < 2 * tid + 2; ++b)
-    if (b < BINS) {
-      const unsigned upto = bins[b] >> COUNT_SHIFT, ahead = b ? bins[b - 1] >> COUNT_SHIFT : 0, after = b < BINS - 1 ? bins[b + 1] >> COUNT_SHIFT : LIST + 1;
-      if (upto <= LIST && after > LIST) fits = b;
-      if (few && upto >= (unsigned)k && ahead < (unsigned)k) reach = b;
-    }
+  unsigned one = 0, two = 0, third = 0;                // tokens of this thread's two bins and of the next
+  if (2 * tid < BINS) {
+    one = bins[2 * tid] >> COUNT_SHIFT;
+    two = bins[2 * tid + 1] >> COUNT_SHIFT;
+    third = 2 * tid + 2 < BINS ? bins[2 * tid + 2] >> COUNT_SHIFT : LIST + 1;
+  }
+  unsigned upto = wave_scan(one + two, Move32{});
+  if ((tid & 63) == 63) count_s[wave] = upto;
+  __syncthreads();
+  upto += below(count_s[tid & 15]);
+  auto look = [&](int b, unsigned ahead, unsigned upto, unsigned after) {
+    if (upto <= LIST && after > LIST) fits = b, fits_count = upto;
+    if (few && upto >= (unsigned)k && ahead < (unsigned)k) reach = b, reach_count = upto;
+  };
+  if (2 * tid < BINS) {
+    look(2 * tid, upto - two - one, upto - two, upto);
+    look(2 * tid + 1, upto - two, upto, upto + third);
+  }
   __syncthreads();
   const int cut = min(fits, reach);
   if (cut >= 0) {
@@ -495,7 +517,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
         for (int e = 0; e < 8; ++e)
           if (v[c].raw(e) >= edge) *at++ = order_key(v[c].raw(e), from + c * CHUNK + e);
   }
-  if (tid == 0) *out = Slice{order_key(top, 0), cut < 0 ? 0 : (int)(bins[cut] >> COUNT_SHIFT), cut};
+  if (tid == 0) *out = Slice{order_key(top, 0), cut < 0 ? 0 : (int)(fits <= reach ? fits_count : reach_count), cut};
 }
 
 // ---- second launch: one workgroup per row finds the token
