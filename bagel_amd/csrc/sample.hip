@@ -6,16 +6,21 @@
 // u x (the kept weights).  A border of one of these sums decides a whole token, so sums have to be better than fp32 and
 // must not depend on the order in which threads come by.
 //
-// No row is sorted.  Tokens are counted into bins of 1/32 octave of weight: with v = 32 log2(e) x / T, token x is in bin
-// floor(v), and weighs 2^(frac(v) / 32), between 1 and 1.022, in that bin's unit, which is computed in 64 bits (to 2^-33) and
-// counted as an integer in steps of 2^-32.  Integer sums are exact in any order, LDS atomics included, and bins and weights
-// depend neither on the maximum nor on how a row is cut up: so the logits are read ONCE, in slices that know nothing of
-// each other, and each slice's histogram reaches 44 octaves below its own maximum (what lies below weighs less than 2^-44 of
-// the first token: nothing).  Where bins are added up, a bin's sum is brought to steps of 2^-42 of the first bin's unit.
+// No row is sorted.  Tokens are counted into bins of 1/32 octave of weight: with v = 32 log2(e) x / T, token x is in the
+// bin of v's nearest whole number r, and weighs 2^((v - r) / 32), between 0.989 and 1.011, in that bin's unit, which is
+// computed in 64 bits (to 2^-33) and counted as an integer in steps of 2^-32.  Integer sums are exact in any order, LDS
+// atomics included, and bins and weights depend neither on the maximum nor on how a row is cut up: so the logits are read
+// ONCE, in slices that know nothing of each other, and each slice's histogram reaches 44 octaves below its own maximum (what
+// lies below weighs less than 2^-44 of the first token: nothing).  Where bins are added up, a bin's sum is brought to steps
+// of 2^-42 of the first bin's unit.
 //
 // Two launches.  The first: a workgroup per slice, whose logits stay in registers: maximum, histogram, and a list of the
-// slice's foremost tokens as (value, index) keys of 64 bits.  Bound by its instructions and LDS atomics, some twenty and one a
-// logit: a bin's count and weight are the two parts of one 64-bit word.  The second: one workgroup per row, in one of three ways:
+// slice's foremost tokens as (value, index) keys of 64 bits.  Bound by its vector instructions (busy 4/5 of the time), some
+// forty a logit and thread: 14 for bin and weight, 10 where tokens are listed, the rest once per slice.  A bin's count and weight
+// are the two parts of one 64-bit word, so that a logit is one LDS atomic.  Measured: 256 rows of 151936 32-bit logits, 156 MB,
+// 54 us = 2.9 TB/s; 64 rows of 152064 bf16 ones, 19 MB, 17.6 us; a single such row 5.6 us.
+// The second (10 us for a row whose borders are listed, 32 us for 64 rows with borders everywhere): one workgroup per row, in one
+// of three ways:
 //   - a top-k of a few: the lists hold it, whatever the row's weights are, so the first launch only counted tokens (without weights),
 //     and the listed tokens are sorted;
 //   - a top-p whose border lies among the listed tokens: they are sorted, and everything else is prefix sums over them;
@@ -70,12 +75,28 @@ __device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }
 // Ascending in the order of the tokens: descending value (the two zeros are one), then ascending index.
 __device__ __forceinline__ u64 order_key(float x, int i) {
   const unsigned b = __float_as_uint(x + 0.0f);
-  const unsigned up = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
-  return ((u64)~up << 32) | (unsigned)i;
+  return ((u64)((int)b < 0 ? b : b ^ 0x7fffffffu) << 32) | (unsigned)i;
 }
 __device__ __forceinline__ float key_value(u64 key) {
   const unsigned up = ~(unsigned)(key >> 32);
   return __uint_as_float(up ^ ((up >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+// The number of x's bin, and `part`, its v less that number: one fused multiply-add with 1.5 x 2^52 leaves the whole number
+// nearest v in the sum's low bits (of x on a border the same one everywhere: nothing is rounded before).
+constexpr double WHOLE = 6755399441055744.0;
+__device__ __forceinline__ double bin_number(float x, double per, double& part) {
+#pragma clang fp contract(off)
+  const double v = (double)x * per;
+  const bool small = __builtin_fabs(v) < 1125899906842624.0;      // 2^50
+  const double near = __builtin_fma((double)x, per, WHOLE) - WHOLE, far = __builtin_rint(v);
+  const double p = __builtin_fma((double)x, per, -near), q = v - far;
+  part = small ? p : q;
+  return small ? near : far;
+}
+__device__ __forceinline__ double bin_number(float x, double per) {
+  double part;
+  return bin_number(x, per, part);
 }
 
 // Bins counted down from that of a maximum `top`.
@@ -83,21 +104,18 @@ struct Scale {
   float top;
   double per;        // 32 log2(e) / T
   double inverse;    // of it, or nearly
-  double base;       // bin of the maximum
+  double base;       // number of the maximum's bin
 };
 constexpr double LN2 = 0.69314718055994530942;
 __device__ __forceinline__ double per_unit(float t) { return OCTAVE / LN2 / (double)t; }
 __device__ __forceinline__ Scale make_scale(float top, float t, double per) {
-#pragma clang fp contract(off)
-  return Scale{top, per, (double)t * (LN2 / OCTAVE), __builtin_floor((double)top * per)};
+  return Scale{top, per, (double)t * (LN2 / OCTAVE), bin_number(top, per)};
 }
 __device__ __forceinline__ Scale make_scale(float top, float t) { return make_scale(top, t, per_unit(t)); }
-// Token x's bin, BINS for one that weighs nothing, and `part` = v - floor(v).  The maximum is in bin 0 even where v is no
-// number (an infinite maximum, an infinite T).
+// Token x's bin, BINS for one that weighs nothing, and `part`.  The maximum is in bin 0 even where v is no number (an
+// infinite maximum, an infinite T).
 __device__ __forceinline__ int bin_of(float x, const Scale& s, double& part) {
-#pragma clang fp contract(off)
-  const double v = (double)x * s.per, d = s.base - __builtin_floor(v);
-  part = __builtin_amdgcn_fract(v);
+  const double d = s.base - bin_number(x, s.per, part);
   if (x == s.top) {
     part = part == part ? part : 0.0;
     return 0;
@@ -121,22 +139,24 @@ __device__ __forceinline__ float edge_of(int b, const Scale& s) {
   if (s.top == INFINITY) return s.top;
   if (!(s.per > 0.0)) return -3.402823466e38f;      // an infinite T: every value is in the maximum's bin
   const double lowest = s.base - b;
-  const float x = next((float)(lowest * s.inverse), (int)(threadIdx.x & 63) - 32);
-  const u64 inside = __ballot((double)x * s.per >= lowest);      // false for what lies below -inf in the bits' order: NaN
+  const float x = next((float)((lowest - 0.5) * s.inverse), (int)(threadIdx.x & 63) - 32);
+  const u64 inside = __ballot(bin_number(x, s.per) >= lowest);      // false for what lies below -inf in the bits' order: NaN
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), inside ? __ffsll(inside) - 1 : 63));
 }
-// 2^(part / 32) in steps: a cubic through its values at the four Chebyshev points of [0, 1] (7e-11 of it off at most); a sum
+// 2^(part / 32) in steps: a cubic through its values at the four Chebyshev points of [-1/2, 1/2] (8e-11 of it off at most); a sum
 // with 2^52 leaves the rounded steps in the low bits.
 struct Cubic {
-  double c3 = 1.71230584268166556e-06 * (1ull << STEPS_LOG2), c2 = 2.34584642666360913e-04 * (1ull << STEPS_LOG2);
-  double c1 = 2.16608517052938078e-02 * (1ull << STEPS_LOG2), c0 = 9.99999999927715377e-01 * (1ull << STEPS_LOG2) + 4503599627370496.0;
-  // kept in scalar registers: otherwise every use first copies them to vector registers
-  __device__ __forceinline__ void settle() { asm volatile("" : "+s"(c3), "+s"(c2), "+s"(c1), "+s"(c0)); }
-  __device__ __forceinline__ u64 steps(double part) const {
+  double c3 = 1.693860906736419904e-06 * (1ull << STEPS_LOG2), c2 = 2.345984913507675400e-04 * (1ull << STEPS_LOG2);
+  double c1 = 2.166084939218784396e-02 * (1ull << STEPS_LOG2), c0 = 9.999999999283390737e-01 * (1ull << STEPS_LOG2) + 4503599627370496.0;
+  double whole = WHOLE;
+  // kept in registers, only one of an instruction's two constants in scalar ones: otherwise every use copies them first
+  __device__ __forceinline__ void settle() { asm volatile("" : "+v"(c3), "+s"(c2), "+s"(c1), "+s"(c0), "+v"(whole)); }
+  // and `more` (a multiple of 2^32) on top
+  __device__ __forceinline__ u64 steps(double part, u64 more = 0) const {
     double p = __builtin_fma(part, c3, c2);
     p = __builtin_fma(p, part, c1);
     p = __builtin_fma(p, part, c0);
-    return (u64)__double_as_longlong(p) & ((1ull << 52) - 1);
+    return (u64)__double_as_longlong(p) + (more - 0x4330000000000000ull);
   }
 };
 __device__ __forceinline__ u64 steps_of(double part) { return Cubic().steps(part); }
@@ -410,7 +430,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = fmaxf(top, v[c].at(e));
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, v[c].raw(e));      // passes over NaN
   top = wave_max(top);
   if ((tid & 63) == 0) top_s[wave] = top;
   __syncthreads();
@@ -449,10 +469,10 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const double y = (double)fmaxf(v[c].raw(e), low) * s.per;
-          const int b = base - (int)__builtin_floor(y);
+          const double x = fmaxf(v[c].raw(e), low), whole = __builtin_fma(x, s.per, cubic.whole);
+          const int b = base - (int)__double_as_longlong(whole);
           if (b < BINS) {
-            if constexpr (weights.value) atomicAdd(&bins[b], ONE + cubic.steps(__builtin_amdgcn_fract(y)));
+            if constexpr (weights.value) atomicAdd(&bins[b], cubic.steps(__builtin_fma(x, s.per, WHOLE - whole), ONE));
             else atomicAdd(&bins[b], ONE);
           }
         }
@@ -508,14 +528,18 @@ __global__ __launch_bounds__(THREADS, 8) void sample_slice_kernel(Params p) {
     unsigned base = 0;
     if ((tid & 63) == 63 && upto) base = atomicAdd(&listed, upto);
     base = __builtin_amdgcn_readlane(base, 63) + upto - mine;
-    u64* at = p.list + ((long)row * p.slices + slice) * LIST + base;
+    char* at = (char*)(p.list + ((long)row * p.slices + slice) * LIST);
+    unsigned to = 8 * base;
     settle();
     if (mine && base + mine <= LIST)                  // always: cut is a bin that fits
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (v[c].raw(e) >= edge) *at++ = order_key(v[c].raw(e), from + c * CHUNK + e);
+          if (v[c].raw(e) >= edge) {
+            *(u64*)(at + to) = order_key(v[c].raw(e), from + c * CHUNK + e);
+            to += 8;
+          }
   }
   if (tid == 0) *out = Slice{order_key(top, 0), cut < 0 ? 0 : (int)(fits <= reach ? fits_count : reach_count), cut};
 }
@@ -921,7 +945,7 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
   if (tid == 0) answer(h.key, kept);
 }
 
-// Chunks per slice: two workgroups share a CU, and one takes about 5 us + 1.6 us a chunk (2 chunks 8.3 us); whole rounds of
+// Chunks per slice: two workgroups share a CU, and one takes about 4.5 us + 1.5 us a chunk (2 chunks 7.5 us); whole rounds of
 // all CUs count.
 int slices_of(int n, int chunks) { return (n + chunks * CHUNK - 1) / (chunks * CHUNK); }
 int chunks_of(int rows, int n, int f32) {
