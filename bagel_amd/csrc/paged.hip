@@ -37,7 +37,7 @@ __device__ __forceinline__ unsigned pack_e4m3(float a, float b, float c, float d
 // each), so a head's norm and its rotation partner stay inside those lanes.  Everything is one pass, bound by memory: each projected
 // element is read once and each result written once.  A thread takes G neighbouring heads of its row, whose loads are in
 // flight together and which share the row's slot and rotation; G = 1 where there are too few rows to fill the chip with four.
-// Many rows (G = 4) pass the caches by: 32768 rows of 36 heads of 128, 621 MB, take 113 us = 5.5 TB/s (121 us through the
+// Many rows (G = 4) pass the caches by: 32768 rows of 36 heads of 128, 621 MB, take 107 us = 5.8 TB/s (121 us through the
 // caches, 144 us with one head per thread; a large copy reaches 4.9 TB/s).
 // ---------------------------------------------------------------------------------------------------------------------
 struct AppendParams {
@@ -157,9 +157,9 @@ int launch_append(const AppendParams& p, hipStream_t st) {
 // than one chunk is split over workgroups; each leaves an unnormalised partial (sums in fp32) and the last one to finish
 // joins them in chunk order, JOIN at a time: more chunks than that are joined in groups first.
 //
-// Bound by the reads of the cache.  28 query and 4 kv heads of 128 (times with the launch): 64 rows of up to 8192 keys, 604 MB
-// of bf16, 108 us = 5.6 TB/s; one row of 131072, 268 MB, 57 us, joins included; e4m3 with 8 kv heads, 200 rows of up
-// to 4096, 475 MB, 94 us = 5.1 TB/s.  Reads of random 16 KB pages alone reach 6.9 TB/s past the caches, 6.0 through them.
+// Bound by the reads of the cache.  28 query and 4 kv heads of 128: 64 rows of up to 8192 keys, 561 MB of bf16, 108 us =
+// 5.2 TB/s; one row of 131072, 268 MB, 55 us = 4.9 TB/s, joins included; e4m3, 200 rows of up to 4096, 476 MB, 93 us = 5.1 TB/s.
+// (Reads of random 16 KB pages alone reach 6.9 TB/s past the caches, 6.0 through them; a large copy 4.9.)
 // Keys straight to registers, 16 bytes of each of 16 rows per lane: 128 us for the first and 115 for the last of these.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int WAVES = 4;
