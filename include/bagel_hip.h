@@ -329,7 +329,7 @@ int bagel_argmax_rows_bf16(const void* logits, long ld, int rows, int n, void* o
  *   min_p:  of these the ones with w_i >= min_p (<= 0: all; always the first)
  *   tokens[row] = the first at which the running sum of the weights kept exceeds uniforms[row] x their sum
  *   logprobs[row] (may be NULL) = ln of its share of the weights kept
- * Weights are computed in 64 bits and counted in whole steps of 2^-33 of themselves or finer, and a weight below 2^-44 of the
+ * Weights are computed in 64 bits and counted in whole steps of 2^-32 of about themselves, and a weight below 2^-44 of the
  * first token's is none; sums of steps are exact, so a row's token does not depend on any order of threads.  temperature
  * <= 0 (or NaN): the first maximum, logprob 0.  NaN logits count as -inf; a row of nothing else gives token 0 with
  * logprob -inf; +inf logits share all the weight.  uniforms outside [0, 1) act as the nearer end, a NaN as 0.
