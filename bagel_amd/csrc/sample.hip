@@ -555,12 +555,12 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
   __shared__ u64 mass[BINS];                 // steps of bin 0 up to and including a bin
   __shared__ unsigned count[BINS];
   __shared__ u64 work[CAP];                  // the tokens being sorted, or the histogram of a narrowing step
-  const double* table = powers.at;
+  __shared__ double table[OCTAVE];
   __shared__ Sums per_wave[THREADS / 64];
   __shared__ int listed_s[MAX_SLICES];       // tokens in a slice's list
   __shared__ int down[MAX_SLICES];           // a slice's first bin, counted from the row's
   __shared__ int found, lowest_cut, enough;
-  __shared__ unsigned gathered;
+  __shared__ unsigned gathered, inside_s;
   __shared__ u64 best_s, edge_s;
   __shared__ Hit hit_s;
   u64* sub_mass = work;                      // [SUB]
@@ -580,8 +580,10 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
   const float t = row_temperature(p, row), top_p = p.top_p ? p.top_p[row] : 1.0f, min_p = p.min_p ? p.min_p[row] : 0.f, u = p.uniforms[row];
   const int k = row_top_k(p, row);
   const bool few = k >= 1 && k <= FEW;
+  const double power = powers.at[tid % OCTAVE];
   if (tid == 0) best_s = ~0ull, lowest_cut = BINS, enough = 1, gathered = 0;
   __syncthreads();
+  if (tid < OCTAVE) table[tid] = power;
   if (tid < MAX_SLICES) {
     const u64 m = wave_min(mine.best);
     if ((tid & 63) == 0) atomicMin(&best_s, m);
@@ -605,7 +607,9 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
     const int b = place(key, part);
     return b < BINS ? scaled(steps_of(part), b, table) : 0ull;
   };
-  const u64 top_steps = steps(best);
+  double top_part;
+  place(best, top_part);
+  const u64 top_steps = steps_of(top_part) << FINER;        // scaled() for bin 0
   if (tid == 0) hit_s = Hit{best, top_steps};
   if (tid < MAX_SLICES) {
     const float their = key_value(mine.best);
@@ -766,15 +770,30 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
   };
   if (few && enough) {
     // of the slices' first k only those in the bins of the row's first k (or all, where that many weigh nothing)
-    for (int b = tid; b < BINS; b += THREADS) mass[b] = 0;
+    for (int b = tid; b < BINS; b += THREADS) count[b] = 0;
+    if (tid == 0) found = BINS;
     __syncthreads();
     for_listed([&](u64 key) {
       const int b = bin_of(key_value(key), s);
-      if (b < BINS) atomicAdd(&mass[b], 1ull);
+      if (b < BINS) atomicAdd(&count[b], 1u);
     });
-    prefix<BINS>(mass, per_wave);
-    const int b = min(find(BINS, [&](int b) { return (b == 0 || mass[b - 1] < (u64)k) && mass[b] >= (u64)k; }), BINS - 1);
-    if (mass[b] <= CAP) {
+    __syncthreads();
+    unsigned one = 0, two = 0;                           // tokens of this thread's two bins
+    if (2 * tid < BINS) one = count[2 * tid], two = count[2 * tid + 1];
+    unsigned upto = wave_scan(one + two, Move32{});
+    if ((tid & 63) == 63) per_wave[tid >> 6].count = upto;
+    __syncthreads();
+    upto += below(per_wave[tid & 15].count);
+    if (upto >= (unsigned)k && upto - two - one < (unsigned)k) {
+      const bool first = upto - two >= (unsigned)k;
+      found = first ? 2 * tid : 2 * tid + 1;
+      inside_s = first ? upto - two : upto;
+    } else if (tid == THREADS - 1 && upto < (unsigned)k) {
+      inside_s = upto;
+    }
+    __syncthreads();
+    const int b = min(found, BINS - 1);
+    if (inside_s <= CAP) {
       const float edge = edge_of(b, s);
       for_listed([&](u64 key) {
         if (key_value(key) >= edge) put(key);
@@ -946,7 +965,7 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
 }
 
 // Chunks per slice: two workgroups share a CU, and one takes about 4.5 us + 1.5 us a chunk (2 chunks 7.5 us); whole rounds of
-// all CUs count.
+// all CUs count.  The second launch waits once more, 2 us, for every ten slices of a row.
 int slices_of(int n, int chunks) { return (n + chunks * CHUNK - 1) / (chunks * CHUNK); }
 int chunks_of(int rows, int n, int f32) {
   const int most = f32 ? 2 : 4;        // 16 registers of logits: with twice as many, two workgroups no longer fit a CU
@@ -954,7 +973,8 @@ int chunks_of(int rows, int n, int f32) {
   long least = 0;
   for (int c = most; c >= 1 && slices_of(n, c) <= MAX_SLICES; c /= 2) {
     const long rounds = ((long)rows * slices_of(n, c) + 2 * bagel_cu_count() - 1) / (2 * bagel_cu_count());
-    if (c == most || rounds * (3 + c) < least) best = c, least = rounds * (3 + c);
+    const long time = 3 * rounds * (3 + c) + 4 * ((slices_of(n, c) + 9) / 10);        // in half microseconds
+    if (c == most || time < least) best = c, least = time;
   }
   return best;
 }
