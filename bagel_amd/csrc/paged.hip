@@ -165,6 +165,7 @@ int launch_append(const AppendParams& p, hipStream_t st) {
 constexpr int WAVES = 4;
 constexpr int JOIN = 16;             // partials that are joined at once
 constexpr int MAX_SPLITS = 8 * JOIN;
+constexpr int SHORT = 512;           // keys that take as long as a level of joins
 constexpr int TICKETS = 16;          // per (row, kv head, head block): one for all chunks or groups of them, eight for the groups
 
 // Blocks of 32 keys per tile: 8 KB of keys and as much of values, half of that for the shortest rows.
@@ -584,14 +585,17 @@ Pool k_pool(const bagel_paged_cache* c) { return pool_of(c->k, c->k_page_stride,
 Pool v_pool(const bagel_paged_cache* c) { return pool_of(c->v, c->v_page_stride, c->v_slot_stride, c->v_head_stride, c->v_scale, c->e4m3); }
 
 // Chunks that rows are split into where none has more than max_kv_len keys: whole rounds of the waves' tiles, two workgroups
-// per CU.
+// per CU.  A level of joins takes 3 to 4 us, about as long as a workgroup takes for 512 keys: rows up to there are not split, and
+// rows of up to JOIN times as many into no more chunks than one level joins.  One row of 28 / 4 heads of 128 in bf16, so and with a
+// chunk per round: 500 keys 6.4 and 7.6 us, 3000 9.2 and 12.3, 8192 13.1 and 13.6 (four rows: 17.9 and 22.0).
 struct Split {
   int splits, chunk;
 };
 long head_blocks(int Hq, int Hkv) { return Hkv * (long)((Hq / Hkv + 15) / 16); }
 long attend_round(int D, int e4m3) { return WAVES * 32 * (D * (e4m3 ? 1 : 2) == 256 ? 1 : 2); }
 Split attend_split(long rows, int Hq, int Hkv, int D, int e4m3, long max_kv_len) {
-  const long want = std::max(1L, std::min<long>(MAX_SPLITS, 2L * bagel_cu_count() / (rows * head_blocks(Hq, Hkv))));
+  const long most = max_kv_len <= SHORT ? 1 : max_kv_len <= SHORT * JOIN ? JOIN : MAX_SPLITS;
+  const long want = std::max(1L, std::min(most, 2L * bagel_cu_count() / (rows * head_blocks(Hq, Hkv))));
   const long round = attend_round(D, e4m3), rounds = std::max(1L, (max_kv_len + round - 1) / round);
   const long chunk = (rounds + want - 1) / want * round;
   return Split{(int)std::max(1L, (max_kv_len + chunk - 1) / chunk), (int)chunk};
