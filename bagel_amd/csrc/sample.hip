@@ -971,7 +971,7 @@ int chunks_of(int rows, int n, int f32) {
   const int most = f32 ? 2 : 4;        // 16 registers of logits: with twice as many, two workgroups no longer fit a CU
   int best = most;
   long least = 0;
-  for (int c = most; c >= 1 && slices_of(n, c) <= MAX_SLICES; c /= 2) {
+  for (int c = most; c >= 1 && slices_of(n, c) <= MAX_SLICES; --c) {
     const long rounds = ((long)rows * slices_of(n, c) + 2 * bagel_cu_count() - 1) / (2 * bagel_cu_count());
     const long time = 3 * rounds * (3 + c) + 4 * ((slices_of(n, c) + 9) / 10);        // in half microseconds
     if (c == most || time < least) best = c, least = time;
@@ -1023,6 +1023,7 @@ extern "C" int bagel_sample_rows(const void* logits, long ld, int rows, int n, i
     hipLaunchKernelGGL(sample_pick_kernel<float>, dim3(rows), block, 0, st, p);
   } else {
     if (c == 4) hipLaunchKernelGGL((sample_slice_kernel<bf16, 4>), grid, block, 0, st, p);
+    else if (c == 3) hipLaunchKernelGGL((sample_slice_kernel<bf16, 3>), grid, block, 0, st, p);
     else if (c == 2) hipLaunchKernelGGL((sample_slice_kernel<bf16, 2>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((sample_slice_kernel<bf16, 1>), grid, block, 0, st, p);
     hipLaunchKernelGGL(sample_pick_kernel<bf16>, dim3(rows), block, 0, st, p);
