@@ -967,8 +967,8 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
 // Chunks per slice: two workgroups share a CU, and one takes about 4.5 us + 1.5 us a chunk (2 chunks 7.5 us); whole rounds of
 // all CUs count.  The second launch waits once more, 2 us, for every ten slices of a row.
 int slices_of(int n, int chunks) { return (n + chunks * CHUNK - 1) / (chunks * CHUNK); }
-int chunks_of(int rows, int n, int f32) {
-  const int most = f32 ? 2 : 4;        // 16 registers of logits: with twice as many, two workgroups no longer fit a CU
+int chunks_of(int rows, int n) {
+  const int most = 4;                  // a slice's steps fit 48 bits, and two workgroups' registers a CU
   int best = most;
   long least = 0;
   for (int c = most; c >= 1 && slices_of(n, c) <= MAX_SLICES; --c) {
@@ -978,10 +978,21 @@ int chunks_of(int rows, int n, int f32) {
   }
   return best;
 }
+template <typename T>
+int launch(const Params& p, int rows, int chunks, hipStream_t st) {
+  const dim3 grid(p.slices, rows), block(THREADS);
+  if (chunks == 4) hipLaunchKernelGGL((sample_slice_kernel<T, 4>), grid, block, 0, st, p);
+  else if (chunks == 3) hipLaunchKernelGGL((sample_slice_kernel<T, 3>), grid, block, 0, st, p);
+  else if (chunks == 2) hipLaunchKernelGGL((sample_slice_kernel<T, 2>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((sample_slice_kernel<T, 1>), grid, block, 0, st, p);
+  hipLaunchKernelGGL(sample_pick_kernel<T>, dim3(rows), block, 0, st, p);
+  BAGEL_LAUNCH_CHECK();
+  return 0;
+}
 // Rows that do not start on 16-byte boundaries reach up to seven places further.
 int places_of(int n) { return n + 7; }
-long workspace_of(int rows, int n, int f32) {
-  return (long)rows * slices_of(places_of(n), chunks_of(rows, places_of(n), f32)) * (sizeof(Slice) + LIST * 8 + BINS * 8);
+long workspace_of(int rows, int n) {
+  return (long)rows * slices_of(places_of(n), chunks_of(rows, places_of(n))) * (sizeof(Slice) + LIST * 8 + BINS * 8);
 }
 
 }  // namespace
@@ -989,7 +1000,7 @@ long workspace_of(int rows, int n, int f32) {
 extern "C" long bagel_sample_rows_workspace_bytes(int rows, int n) {
   long most = 0;       // fewer rows can be cut into more slices altogether
   if (n > 0 && n <= MAX_TOKENS)
-    for (int r = 1; r <= std::min(rows, 65535); ++r) most = std::max(most, std::max(workspace_of(r, n, 0), workspace_of(r, n, 1)));
+    for (int r = 1; r <= std::min(rows, 65535); ++r) most = std::max(most, workspace_of(r, n));
   return most;
 }
 
@@ -1003,31 +1014,18 @@ extern "C" int bagel_sample_rows(const void* logits, long ld, int rows, int n, i
   BAGEL_CHECK(logits && uniforms && tokens && workspace, "bagel_sample_rows: null operand");
   BAGEL_CHECK(ld >= n || ld == 0, "bagel_sample_rows: leading dim %ld below %d tokens", ld, n);
   BAGEL_CHECK((uintptr_t)logits % (logits_f32 ? 4 : 2) == 0 && (uintptr_t)workspace % 16 == 0, "bagel_sample_rows: misaligned operand");
-  const long need = workspace_of(rows, n, logits_f32);
+  const long need = workspace_of(rows, n);
   BAGEL_CHECK(workspace_bytes >= need, "bagel_sample_rows: workspace of %ld bytes, %ld needed", workspace_bytes, need);
   Params p;
   p.logits = logits; p.ld = ld; p.n = n;
   p.uniforms = (const float*)uniforms; p.temperature = (const float*)temperature; p.top_k = (const int*)top_k;
   p.top_p = (const float*)top_p; p.min_p = (const float*)min_p; p.tokens = (int*)tokens; p.logprobs = (float*)logprobs;
-  const int c = chunks_of(rows, places_of(n), logits_f32);
+  const int c = chunks_of(rows, places_of(n));
   p.slices = slices_of(places_of(n), c);
   const long slices = (long)rows * p.slices;
   p.slice = (Slice*)workspace;
   p.list = (u64*)(p.slice + slices);
   p.bins = p.list + slices * LIST;
-  const dim3 grid(p.slices, rows), block(THREADS);
   hipStream_t st = (hipStream_t)stream;
-  if (logits_f32) {
-    if (c == 2) hipLaunchKernelGGL((sample_slice_kernel<float, 2>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((sample_slice_kernel<float, 1>), grid, block, 0, st, p);
-    hipLaunchKernelGGL(sample_pick_kernel<float>, dim3(rows), block, 0, st, p);
-  } else {
-    if (c == 4) hipLaunchKernelGGL((sample_slice_kernel<bf16, 4>), grid, block, 0, st, p);
-    else if (c == 3) hipLaunchKernelGGL((sample_slice_kernel<bf16, 3>), grid, block, 0, st, p);
-    else if (c == 2) hipLaunchKernelGGL((sample_slice_kernel<bf16, 2>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((sample_slice_kernel<bf16, 1>), grid, block, 0, st, p);
-    hipLaunchKernelGGL(sample_pick_kernel<bf16>, dim3(rows), block, 0, st, p);
-  }
-  BAGEL_LAUNCH_CHECK();
-  return 0;
+  return logits_f32 ? launch<float>(p, rows, c, st) : launch<bf16>(p, rows, c, st);
 }
