@@ -149,8 +149,12 @@ int launch_append(const AppendParams& p, hipStream_t st) {
 //   - V rows go to registers (16 lanes x D / 16 elements, 8 keys per lane group).  The operand wants 8 KEYS of one d per
 //     lane; the lane has D / 16 d's of those 8 keys, so byte permutes turn one into the other inside the lane, and
 //     row r of product dd is d = (D / 16) r + dd.
-// The softmax is the running form: one maximum and sum per head and wave, scores and sums in fp32, P rounded to bf16 for
-// the matrix product (an error of 2^-9 of each weight, which the output's own rounding to bf16 exceeds).
+// The softmax is the running form: one maximum and sum per head and wave, scores and sums in fp32.  The matrix product takes P as the
+// sum of two bf16 parts: the next bf16 number below the weight, and what that leaves, which is positive (a value of infinity
+// times a part of zero would be NaN).  e4m3 has no infinity, so there the first part is the weight rounded, in fewer instructions.
+// Together they are within 2^-15 of each weight, so the output's rounding is the only one to bf16 that shows; one rounded part alone
+// is off by up to 2^-8, as much as the output's rounding, and by far more where values cancel.  What the second part costs (us, one
+// part and two): 64 rows of up to 8192 bf16 keys, slots first, 121.0 and 121.5, 200 rows of e4m3 94.6 and 95.4, one row of 131072 53.7 and 53.4.
 // An e4m3 value is a bf16 value: keys and values are widened exactly, the scales enter in fp32.
 //
 // One workgroup = four waves that take turns at the chunk's tiles, each with its own running softmax.  A row with more keys
@@ -211,8 +215,10 @@ __device__ __forceinline__ float column_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Three waves per SIMD: at most 168 registers, and the compiler takes 167 (bf16 at D = 128) without being held to it; held to it, it
+// spills two of them.
 template <int D, bool F8>
-__global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendParams p) {
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_attention_kernel(AttendParams p) {
   constexpr int ITEM = F8 ? 1 : 2;
   constexpr int SUB = tile_blocks<D, F8>();    // blocks of 32 keys per tile
   constexpr int TK = 32 * SUB;                 // keys per tile
@@ -375,12 +381,30 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
     for (int i = 0; i < ND; ++i) acc[i] *= alpha;
 #pragma unroll
     for (int b = 0; b < SUB; ++b) {
-      bf16x8 pb;
+      u32x4 most;
+      bf16x8 rest;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float w = __builtin_amdgcn_exp2f(s[b][e] - m_new);
-        l_run += w;
-        pb[e] = (bf16)w;
+      for (int e = 0; e < 8; e += 2) {
+        float w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          w[i] = __builtin_amdgcn_exp2f(s[b][e + i] - m_new);
+          l_run += w[i];
+        }
+        if constexpr (F8) {
+          const bf16x2 r = {(bf16)w[0], (bf16)w[1]};
+          most[e / 2] = __builtin_bit_cast(unsigned, r);
+          rest[e] = (bf16)(w[0] - __uint_as_float(most[e / 2] << 16));
+          rest[e + 1] = (bf16)(w[1] - __uint_as_float(most[e / 2] & 0xffff0000u));
+        } else {
+          unsigned below[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            below[i] = __builtin_elementwise_sub_sat(__float_as_uint(w[i]), 1u);
+            rest[e + i] = (bf16)(w[i] - __uint_as_float(below[i] & 0xffff0000u));      // exact before its rounding
+          }
+          most[e / 2] = __builtin_amdgcn_perm(below[1], below[0], 0x07060302u);
+        }
       }
 #pragma unroll
       for (int dd = 0; dd < ND; ++dd) {
@@ -396,7 +420,8 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attention_kernel(AttendPa
             a[i] = __builtin_amdgcn_perm(x.v[b][2 * i + 1][dd / 2], x.v[b][2 * i][dd / 2], dd % 2 ? 0x07060302u : 0x05040100u);
           }
         }
-        acc[dd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), pb, acc[dd], 0, 0, 0);
+        acc[dd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), rest, acc[dd], 0, 0, 0);
+        acc[dd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, most), acc[dd], 0, 0, 0);
       }
     }
   };

@@ -477,3 +477,52 @@ def test_attention_joins_in_groups(n, rows, hq, hkv, d, dtype):
     first = c.run(ws=ws).clone()
     c.check()
     assert torch.equal(c.run(ws=ws), first) and not bool(ws[:16384].any())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F8])
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (6, 3, 64), (17, 1, 64)])
+@pytest.mark.parametrize("lens", [[2, 0, 64, 130, 1000, 5000], [33000]])
+def test_attention_keeps_the_weights_bits(lens, hq, hkv, d, dtype):
+    """Values that nearly cancel show the rounding of the weights: every second key weighs a little less than the one before it
+    and has its value with the other sign, so that a head's result is a small difference of two large sums."""
+    c = _Case(lens, hq, hkv, d, 16, dtype, "slots first", seed=31)
+    a = (1 + torch.rand((hkv, d), device=DEV, generator=c.gen) * 15).to(F8).float()         # numbers of either type
+    for r, n in enumerate(lens):
+        at = torch.arange(n, device=DEV)
+        pages, slots = c.table[r].long()[at // 16], at % 16
+        k = torch.zeros((n, hkv, d), device=DEV)
+        k[::2, :, 0] = 1.0
+        v = torch.where((at % 2 == 0)[:, None, None], a, -a)
+        raw = torch.uint8 if dtype == F8 else torch.int16
+        for pool, x in ((c.kp, k), (c.vp, v)):
+            pool.view(raw)[pages, slots] = x.to(dtype).view(raw)
+    step = 1.0 if c.ks is None else float(c.ks.min())
+    c.q.zero_()
+    c.q[:, :, 0] = ((0.01 + 0.4 * torch.rand(c.q.shape[:2], device=DEV, generator=c.gen)) * d ** 0.5 / step).to(BF16)
+    c.run()
+    want, mag = c.want()
+    # a score is one product, below 1.3: in 32 bits with its scale off by less than 2^-21, and so is the exponential; the weights
+    # as two bf16 parts are off by half a step of the second (2^-8), which is a step of the first at most (2^-7); sums and the
+    # scale of the values by less than 2^-19
+    tol = HALF_STEP[BF16] * want.abs() + (2.0 ** -15 + 2.0 ** -18) * mag
+    got = c.out().double()
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / mag.clamp(min=1e-9)).max())
+
+
+def test_attention_of_infinite_values():
+    """An infinite value makes its element infinite and no other, whatever its weight: a whole one, a single key's or a small one."""
+    n = 96
+    c = _Case([n] * n, 4, 2, 64, 16, BF16, "slots first", seed=32)
+    c.table[:, :n // 16] = torch.arange(n * n // 16, device=DEV, dtype=torch.int32).view(n, -1)     # every page is some row's
+    c.kp.copy_(_normal(c.kp.shape, c.gen))
+    c.vp.copy_(_normal(c.vp.shape, c.gen))
+    c.q.copy_(_normal(c.q.shape, c.gen, 0.5))
+    c.q[::3] = 0.0                                                   # every weight 1
+    want = torch.zeros((n, 4, 64), device=DEV)
+    for r in range(n):
+        sign = -1.0 if r % 2 else 1.0
+        c.vp[int(c.table[r, r // 16]), r % 16, 1, r % 64] = sign * math.inf
+        want[r, 2:, r % 64] = sign * math.inf
+    c.run()
+    got = c.out().float()
+    assert torch.equal(torch.where(torch.isfinite(got), 0.0, got), want)
