@@ -941,22 +941,38 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
   if (min_p > 0.f) {
     // the threshold's bin, and one to each side for the roundings at the bins' borders: only their tokens are looked at
     const double edge = -log((double)min_p) * (OCTAVE / LN2);
-    const int b0 = edge < 2.0 ? 0 : edge < BINS ? (int)edge - 2 : BINS, b1 = b0 + 5;
+    constexpr int LOOK = 6;
+    const int b0 = edge < 2.0 ? 0 : edge < BINS ? (int)edge - 2 : BINS, b1 = b0 + LOOK - 1;
     if (b0 < BINS && (border.key == ~0ull || bin_of(key_value(border.key), s) >= b0)) {
-      u64 sum = 0;
+      // by bin, so that the sum of what stays is rounded as resolve() rounds it and a draw of all of it ends at its last token
+      u64 sum[LOOK] = {};
+      __syncthreads();
+      if (tid < LOOK) work[tid] = 0;
+      __syncthreads();
       const float least = edge_of(min(b1, BINS - 1), s), beyond = b0 ? edge_of(b0 - 1, s) : __builtin_nanf("");
       auto add = [&](u64 key) {
-        if (key <= border.key && weight(key_value(key)) >= (double)min_p) sum += steps(key);
+        if (!(key <= border.key && weight(key_value(key)) >= (double)min_p)) return;
+        double part;
+        const int b = place(key, part);
+        const u64 mine = steps_of(part);
+#pragma unroll
+        for (int i = 0; i < LOOK; ++i) sum[i] += b == b0 + i ? mine : 0;
       };
       if (b1 <= lowest_cut) for_listed([&](u64 key) {
         if (key_value(key) >= least && !(key_value(key) >= beyond)) add(key);
       });
       else for_range<T>(p, row, least, beyond, [&](float x, int i) { add(order_key(x, i)); });
+#pragma unroll
+      for (int i = 0; i < LOOK; ++i) {
+        const u64 all = wave_scan(sum[i]);
+        if ((tid & 63) == 63 && all) atomicAdd(&work[i], all);
+      }
       __syncthreads();
-      const Sums v = scan(Sums{sum, 0}, per_wave);
-      if (tid == THREADS - 1) edge_s = v.mass;
+      int last = LOOK - 1;                               // the last bin with a token that stays; all of those before it do
+      while (last > 0 && !work[last]) --last;
+      const int b = b0 + last;
+      kept = max((b ? mass[b - 1] : 0) + scaled(work[last], b, table), top_steps);     // the first token stays whatever min_p is
       __syncthreads();
-      kept = max((b0 ? mass[b0 - 1] : 0) + edge_s, top_steps);         // the first token stays whatever min_p is
     }
   }
   const u64 target = u_target(kept);

@@ -268,3 +268,24 @@ def test_sampling_captured():
         token, logprob = _want(x, **s)
         assert torch.equal(tokens.long(), token)
         assert math.isfinite(float(logprobs.sum())) and bool(((logprobs.double() - logprob).abs() <= 2.0 ** -24 * logprob.abs() + 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("change", [dict(k=0, p=1.0), dict(k=0, p=0.999), dict(k=9000, p=1.0), dict(k=9000, p=0.999)])
+@pytest.mark.parametrize("n", [20000, 152064])
+def test_sampling_of_the_last_token_above_min_p(n, change, dtype):
+    """A uniform at or beyond 1 draws the last token that the filters keep, and none that min-p leaves out, also where min-p's
+    border lies among thousands of tokens of nearly its weight."""
+    gen = torch.Generator(device=DEV).manual_seed(21)
+    rows = 48
+    x = torch.randn((rows, n), device=DEV, generator=gen).to(dtype)
+    s = _settings(rows, gen, t=1.0, **change)
+    s["m"] = 10.0 ** (-1 - 3 * torch.rand(rows, device=DEV, generator=gen))
+    for u in (1.0, 3.0, INF):
+        want = _want(x, torch.ones(rows, device=DEV), s["t"], s["k"], s["p"], s["m"])[0]
+        K = _K()
+        ws = torch.zeros(K.sample_rows_workspace_bytes(rows, n), device=DEV, dtype=torch.uint8)
+        tokens = torch.empty(rows, device=DEV, dtype=torch.int32)
+        K.sample_rows(x, torch.full((rows,), u, device=DEV), tokens, ws, temperature=s["t"], top_k=s["k"], top_p=s["p"], min_p=s["m"])
+        off = torch.nonzero(tokens.long() != want)[:, 0].tolist()
+        assert not off, (u, len(off), [(r, int(tokens[r]), int(want[r])) for r in off[:4]])
