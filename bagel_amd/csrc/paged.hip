@@ -36,9 +36,9 @@ __device__ __forceinline__ unsigned pack_e4m3(float a, float b, float c, float d
 // Append.  Row r of qkv holds Hq query heads, Hkv key heads and Hkv value heads of D; D / 8 lanes hold a head (16 bytes
 // each), so a head's norm and its rotation partner stay inside those lanes.  Everything is one pass, bound by memory: each projected
 // element is read once and each result written once.  A thread takes G neighbouring heads of its row, whose loads are in
-// flight together and which share the row's slot and rotation; G = 1 where there are too few rows to fill the chip with four.
+// flight together and which share the row's slot and rotation; G = 1 where there are too few rows (launch_append).
 // Many rows (G = 4) pass the caches by: 32768 rows of 36 heads of 128, 621 MB, take 107 us = 5.8 TB/s (121 us through the
-// caches, 144 us with one head per thread; a large copy reaches 4.9 TB/s).
+// caches, 138 us with one head per thread; a large copy reaches 4.9 TB/s); the same into e4m3 pages, 554 MB, 146 us.
 // ---------------------------------------------------------------------------------------------------------------------
 struct AppendParams {
   const bf16* qkv;
@@ -125,8 +125,15 @@ template <int D, bool F8>
 int launch_append(const AppendParams& p, hipStream_t st) {
   constexpr int LPH = D / 8, PER_BLOCK = 256 / LPH;
   const int heads = p.Hq + 2 * p.Hkv;
-  // four heads per thread once that still gives every CU eight workgroups (36 heads: from 910 rows on)
-  const int g = (long)p.rows * ((heads + 3) / 4) >= 8L * bagel_cu_count() * PER_BLOCK ? 4 : 1;
+  // Four heads per thread once that still gives every CU four workgroups; in e4m3, whose divisions take longer by the thread, only
+  // where the rows no longer fit the caches that the four-heads form passes by.  Measured (us, one and four heads per thread):
+  //   28 / 4 heads of 128, bf16   1500 rows 9.2 9.9    1820 (four workgroups per CU) 10.7 10.1   2400 13.1 11.5   32768 138 107
+  //   24 / 1 of 128, bf16         1820 rows 8.4 8.8    2400 (four) 10.2 9.6                      6553 22.2 19.2   32768 104 79
+  //   14 / 2 of 64, bf16          4500 rows 8.4 9.1    6553 (four) 10.2 10.1                     8192 12.5 11.1   20000 24.3 23.0
+  //   28 / 4 of 128, e4m3         2400 rows 14.2 16.5  8192 (18) 35.1 41.0                       20000 (44) 97 92   32768 154 146
+  //   32 / 8 of 128, e4m3         8192 rows 44.9 48.5  20000 (59) 127 107                        32768 201 171
+  //   16 / 16 of 64               bf16 8192 rows (12) 22.7 25.2, the worst of the rule, 32768 94 76;   e4m3 20000 rows (29) 60 73, 32768 (48) 115 115
+  const int g = (long)p.rows * ((heads + 3) / 4) >= (F8 ? 40L : 4L) * bagel_cu_count() * PER_BLOCK ? 4 : 1;
   const long blocks = ((long)p.rows * ((heads + g - 1) / g) + PER_BLOCK - 1) / PER_BLOCK;
   BAGEL_CHECK(blocks * PER_BLOCK <= 0x7fffffffL, "bagel_paged_kv_append_bf16: %d rows are too many for one launch", p.rows);
   if (g == 4) hipLaunchKernelGGL((paged_append_kernel<D, F8, 4>), dim3((unsigned)blocks), dim3(256), 0, st, p);
