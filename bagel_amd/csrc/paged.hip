@@ -38,7 +38,7 @@ __device__ __forceinline__ unsigned pack_e4m3(float a, float b, float c, float d
 // element is read once and each result written once.  A thread takes G neighbouring heads of its row, whose loads are in
 // flight together and which share the row's slot and rotation; G = 1 where there are too few rows (launch_append).
 // Many rows (G = 4) pass the caches by: 32768 rows of 36 heads of 128, 621 MB, take 107 us = 5.8 TB/s (121 us through the
-// caches, 138 us with one head per thread; a large copy reaches 4.9 TB/s); the same into e4m3 pages, 554 MB, 146 us.
+// caches, 138 us with one head per thread; a large copy reaches 4.9 TB/s); the same into e4m3 pages, 587 MB, 146 us.
 // ---------------------------------------------------------------------------------------------------------------------
 struct AppendParams {
   const bf16* qkv;

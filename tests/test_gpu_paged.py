@@ -526,3 +526,64 @@ def test_attention_of_infinite_values():
     c.run()
     got = c.out().float()
     assert torch.equal(torch.where(torch.isfinite(got), 0.0, got), want)
+
+
+# Rows from which four heads share a thread: 1024 workgroups of 16 (head_dim 128) or 32 (64) groups of four heads, ten times as many in e4m3
+@pytest.mark.parametrize("rows,hq,hkv,d,page,dtype,order,change", [
+    (1900, 28, 4, 128, 16, BF16, "heads first", dict()),                               # whole groups
+    (2500, 24, 1, 128, 64, BF16, "slots first", dict()),                               # keys begin and end a group, the last is of two
+    (6700, 14, 2, 64, 16, BF16, "padded", dict()),                                     # queries and keys share a group, so do keys and values
+    (8300, 9, 3, 64, 8, BF16, "slots first", dict()),                                  # three heads in the last group
+    (8300, 9, 3, 64, 8, BF16, "slots first", dict(norm=False)), (8300, 9, 3, 64, 8, BF16, "slots first", dict(rope=False)),
+    (22000, 0, 3, 64, 16, BF16, "slots first", dict(with_q=False)), (33500, 5, 2, 64, 16, BF16, "heads first", dict(with_q=False)),
+    (23500, 24, 1, 128, 64, F8, "heads first", dict()), (25000, 21, 3, 128, 16, F8, "slots first", dict(norm=False)),
+    (83000, 9, 3, 64, 16, F8, "padded", dict()), (66500, 14, 2, 64, 128, F8, "heads first", dict(rope=False)),
+    (82500, 0, 8, 64, 128, F8, "slots first", dict(with_q=False))])
+def test_append_of_many_rows(rows, hq, hkv, d, page, dtype, order, change):
+    _append_case(rows, hq, hkv, d, page, dtype, order, seed=rows, **change)
+
+
+@pytest.mark.parametrize("rows,d,hq,hkv", [(3400, 128, 14, 2), (8300, 64, 9, 3)])
+@pytest.mark.parametrize("und_rounding", [False, True])
+def test_append_of_many_rows_in_place(und_rounding, rows, d, hq, hkv):
+    """Queries take the place of their source, bit for bit those of the workspace's scatter, as keys and values are."""
+    K = _K()
+    gen = _gen(9)
+    S = -(-rows // 64) * 64
+    qkv = _normal((rows, (hq + 2 * hkv) * d), gen, 1.5)
+    qw, kw = 1 + _normal((d,), gen, 0.1), 1 + _normal((d,), gen, 0.1)
+    cos, sin = _normal((90, d), gen).cos(), _normal((90, d), gen).sin()
+    cs = torch.randint(0, 90, (rows,), device=DEV, generator=gen, dtype=torch.int32)
+    slots = torch.randperm(S, device=DEV, generator=gen)[:rows].to(torch.int32)
+    Q = torch.zeros((rows, hq, d), device=DEV, dtype=BF16)
+    kws, vws = torch.zeros((hkv, S, d), device=DEV, dtype=BF16), torch.zeros((hkv, d, S), device=DEV, dtype=BF16)
+    K.qk_norm_rope_kv(qkv, rows, hq, hkv, d, qw, qw, kw, kw, rows, cos, sin, cs, slots, Q, kws, vws, S, 1e-6, und_rounding)
+    kp, vp = (torch.zeros((S // 64, 64, hkv, d), device=DEV, dtype=BF16) for _ in range(2))
+    mine = qkv[:, :hq * d].unflatten(1, (hq, d))
+    K.paged_kv_append(qkv, hq, K.PagedCache(kp, vp), slots, Q=mine, q_norm=qw, k_norm=kw, cos_t=cos, sin_t=sin, row_cs=cs, eps=1e-6,
+                      und_rounding=und_rounding)
+    assert torch.equal(mine, Q)
+    assert torch.equal(kp.view(S, hkv, d), kws.transpose(0, 1)) and torch.equal(vp.view(S, hkv, d), vws.permute(2, 0, 1))
+
+
+def test_append_of_many_rows_that_do_not_exist():
+    K = _K()
+    gen = _gen(14)
+    rows, hq, hkv, d, page = 8300, 9, 3, 64, 16
+    qkv = _normal((rows, (hq + 2 * hkv) * d), gen)
+    pages = rows // page + 1
+    kp, vp = (torch.zeros((pages, page, hkv, d), device=DEV, dtype=BF16) for _ in range(2))
+    cos, sin = torch.ones((4, d), device=DEV, dtype=BF16), torch.zeros((4, d), device=DEV, dtype=BF16)
+    slots, cs = torch.arange(rows, device=DEV, dtype=torch.int32), torch.arange(rows, device=DEV, dtype=torch.int32) % 4
+    bad = torch.rand(rows, device=DEV, generator=gen) < 0.3
+    kind = torch.arange(rows, device=DEV) % 4
+    slots[bad & (kind == 0)] = pages * page
+    slots[bad & (kind == 1)] = 2 ** 31 - 1
+    cs[bad & (kind == 2)] = 4
+    cs[bad & (kind == 3)] = -1
+    Q = torch.zeros((rows, hq, d), device=DEV, dtype=BF16)
+    K.paged_kv_append(qkv, hq, K.PagedCache(kp, vp), slots, Q=Q, cos_t=cos, sin_t=sin, row_cs=cs)
+    x = qkv.view(rows, hq + 2 * hkv, d)
+    assert torch.equal(torch.isnan(Q).flatten(1).all(1), bad) and torch.equal(Q[~bad], x[~bad, :hq])
+    for pool, new in ((kp, x[:, hq:hq + hkv]), (vp, x[:, hq + hkv:])):
+        assert torch.equal(pool.view(-1, hkv, d)[:rows], torch.where(bad[:, None, None], 0.0, new).to(BF16))
