@@ -980,16 +980,19 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(Params p) {
   if (tid == 0) answer(h.key, kept);
 }
 
-// Chunks per slice: two workgroups share a CU, and one takes about 4.5 us + 1.5 us a chunk (2 chunks 7.5 us); whole rounds of
-// all CUs count.  The second launch waits once more, 2 us, for every ten slices of a row.
+// Chunks per slice.  A round of one workgroup per CU takes 1.3 us + 1.1 us a chunk, in both types (two share a CU, so a second
+// one beside the first costs as much as one behind it), and whole rounds count; the second launch waits 2 us for every ten slices of a
+// row.  Over 120 sizes, 1 to 600 rows of 5000 to 10^6 tokens, this picks the fastest of the four or one within 3 % of it.  Calls of
+// 1, 2, 3 and 4 chunks (us, bf16; top-k 20): 32 rows of 152064 20.0 17.4 15.2 16.2; 64 of them 24.6 20.3 18.6 20.1; 128 of
+// them 36.4 28.2 28.5 27.7; 128 of 32000 14.6 13.2 14.6 15.5; 32-bit logits, 64 rows of 152064 25.1 22.1 20.8 22.8.
 int slices_of(int n, int chunks) { return (n + chunks * CHUNK - 1) / (chunks * CHUNK); }
 int chunks_of(int rows, int n) {
   const int most = 4;                  // a slice's steps fit 48 bits, and two workgroups' registers a CU
   int best = most;
   long least = 0;
   for (int c = most; c >= 1 && slices_of(n, c) <= MAX_SLICES; --c) {
-    const long rounds = ((long)rows * slices_of(n, c) + 2 * bagel_cu_count() - 1) / (2 * bagel_cu_count());
-    const long time = 3 * rounds * (3 + c) + 4 * ((slices_of(n, c) + 9) / 10);        // in half microseconds
+    const long rounds = ((long)rows * slices_of(n, c) + bagel_cu_count() - 1) / bagel_cu_count();
+    const long time = rounds * (13 + 11 * c) + 20 * ((slices_of(n, c) + 9) / 10);        // in tenths of a microsecond
     if (c == most || time < least) best = c, least = time;
   }
   return best;
