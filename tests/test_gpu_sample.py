@@ -289,3 +289,27 @@ def test_sampling_of_the_last_token_above_min_p(n, change, dtype):
         K.sample_rows(x, torch.full((rows,), u, device=DEV), tokens, ws, temperature=s["t"], top_k=s["k"], top_p=s["p"], min_p=s["m"])
         off = torch.nonzero(tokens.long() != want)[:, 0].tolist()
         assert not off, (u, len(off), [(r, int(tokens[r]), int(want[r])) for r in off[:4]])
+
+
+def _chunks(rows, n, dtype):
+    """Chunks of 8192 logits per slice that a call on these sizes is cut into, from the workspace that its refusal asks for."""
+    import ctypes
+    import re
+    K = _K()
+    a = ctypes.c_void_p(1 << 20)                              # refused before it is followed
+    assert K.lib().bagel_sample_rows(a, K.L(n), K.I(rows), K.I(n), K.I(int(dtype == torch.float32)), a, None, None, None, None, a, None, a, K.L(0), None)
+    need = int(re.search(r"(\d+) needed", K.lib().bagel_last_error().decode()).group(1))
+    slices = need // rows // (16 + 512 * 8 + 1408 * 8)        # a slice's summary, list and bins
+    return [c for c in (1, 2, 3, 4) if -(-(n + 7) // (8192 * c)) == slices]
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("chunks,rows,n", [(1, 9, 60001), (2, 6, 152064), (2, 40, 65537), (3, 64, 65537), (3, 60, 152064), (4, 100, 151936), (2, 260, 32003), (4, 250, 32003),
+                                           (4, 2, 1 << 20)])
+def test_sampling_in_slices_of_every_size(chunks, rows, n, dtype):
+    """One to four chunks per slice, rows of more than ten slices, rows off 16-byte boundaries."""
+    assert chunks in _chunks(rows, n, dtype)
+    gen = torch.Generator(device=DEV).manual_seed(23)
+    x = _logits(rows, n + 3, gen, dtype)[:, 1:n + 1]
+    for change in (dict(k=0, p=0.95, m=0.0), dict(k=20, p=0.8, m=0.0), dict(k=0, p=1.0, m=0.0), dict(t=0.0), dict()):
+        _check(x, **_settings(rows, gen, n=n, **change), what=(chunks, change))
