@@ -45,7 +45,7 @@ struct AppendParams {
   long ld;
   const bf16 *q_w, *k_w, *cos_t, *sin_t;   // norm weights [D], rotation rows [*][D]; null: that step is left out
   const int *row_cs, *row_slot;
-  bf16* Q;                                 // null: queries are not asked for
+  bf16* Q;                                 // null where Hq is 0
   long ldq;
   Pool k, v;
   long capacity;                           // slots in the pool
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
     // a slot or rotation row that does not exist: nothing is stored, and the row's queries say so
 #pragma unroll
     for (int g = 0; g < G; ++g)
-      if (p.Q && first + g < p.Hq) {
+      if (first + g < p.Hq) {
         bf16x8 nan;
 #pragma unroll
         for (int e = 0; e < 8; ++e) nan[e] = (bf16)__builtin_nanf("");
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     const int head = first + g;
-    if (head >= heads || (head < keys && !p.Q)) continue;
+    if (head >= heads) continue;
     float y[8];
     if (head >= values) {
 #pragma unroll
@@ -659,6 +659,10 @@ extern "C" int bagel_paged_kv_append_bf16(const void* qkv, long ld, int rows, in
   BAGEL_CHECK(!Q || (ldq % 8 == 0 && ldq >= (long)Hq * D), "bagel_paged_kv_append_bf16: bad leading dim of Q");
   BAGEL_CHECK(((uintptr_t)qkv | (uintptr_t)Q | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)cos_table | (uintptr_t)sin_table) % 16 == 0,
               "bagel_paged_kv_append_bf16: misaligned operand");
+  if (!Q) {                                      // the heads from the keys on are all there is
+    qkv = (const bf16*)qkv + (long)Hq * D;
+    Hq = 0;
+  }
   AppendParams p;
   p.qkv = (const bf16*)qkv; p.ld = ld; p.q_w = (const bf16*)q_norm; p.k_w = (const bf16*)k_norm;
   p.cos_t = (const bf16*)cos_table; p.sin_t = (const bf16*)sin_table;
