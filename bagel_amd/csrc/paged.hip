@@ -176,6 +176,7 @@ int launch_append(const AppendParams& p, hipStream_t st) {
 constexpr int WAVES = 4;
 constexpr int JOIN = 16;             // partials that are joined at once
 constexpr int MAX_SPLITS = 8 * JOIN;
+constexpr long MAX_KEYS = 1L << 30;  // of a row
 constexpr int SHORT = 512;           // keys that take as long as a level of joins
 constexpr int TICKETS = 16;          // per (row, kv head, head block): one for all chunks or groups of them, eight for the groups
 
@@ -678,6 +679,7 @@ extern "C" int bagel_paged_kv_append_bf16(const void* qkv, long ld, int rows, in
 
 extern "C" long bagel_paged_decode_attention_workspace_bytes(int rows, int Hq, int Hkv, int head_dim, long max_kv_len) {
   if (rows <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0 || max_kv_len < 0) return 0;
+  if (max_kv_len == 0) max_kv_len = MAX_KEYS;
   return ticket_bytes() + std::max(most_partials(rows, Hq, Hkv, head_dim, 0, max_kv_len), most_partials(rows, Hq, Hkv, head_dim, 1, max_kv_len)) *
                               (head_dim + 2) * 4;
 }
@@ -700,7 +702,7 @@ extern "C" int bagel_paged_decode_attention_bf16(const void* Q, long ldq, int ro
   const int blocks = (Hq / Hkv + 15) / 16;
   BAGEL_CHECK((long)Hkv * blocks <= 65535, "bagel_paged_decode_attention_bf16: too many heads");
   const long room = (long)table_width * cache->page_size;
-  BAGEL_CHECK(room <= 1L << 30, "bagel_paged_decode_attention_bf16: a page table of %d pages of %d slots (at most 2^30 keys a row)",
+  BAGEL_CHECK(room <= MAX_KEYS, "bagel_paged_decode_attention_bf16: a page table of %d pages of %d slots (at most 2^30 keys a row)",
               table_width, cache->page_size);
   const long bound = max_kv_len > 0 ? std::min(max_kv_len, room) : room;
   const Split split = attend_split(rows, Hq, Hkv, D, cache->e4m3, bound);

@@ -264,7 +264,7 @@ int bagel_paged_kv_append_bf16(const void* qkv, long ld, int rows, int Hq, const
  * max_kv_len: an upper bound of kv_lens (sizes the split over the length; 0 = unknown, table_width pages; a bound that is too small
  * costs time, not keys).  softmax_scale 0: 1 / sqrt(head_dim).
  * workspace: bagel_paged_decode_attention_workspace_bytes(), which serves every call of this head layout with no more rows
- * and keys; zero before the first call (the tickets at its start, which every call leaves zero);
+ * and keys (max_kv_len 0: any number of keys); zero before the first call (the tickets at its start, which every call leaves zero);
  * calls that share one must not overlap, be they on two streams or in two replayed graphs.  rows <= 65535. */
 long bagel_paged_decode_attention_workspace_bytes(int rows, int Hq, int Hkv, int head_dim, long max_kv_len);
 int bagel_paged_decode_attention_bf16(const void* Q, long ldq, int rows, int Hq, const bagel_paged_cache* cache,

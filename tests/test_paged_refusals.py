@@ -143,3 +143,10 @@ def test_nothing_to_do_is_no_error():
     assert _c_append(_c_cache(), rows=0, qkv=None, slot=None) == 0
     assert _c_attend(_c_cache(), rows=0, q=None, o=None) == 0
     assert K.paged_decode_attention_workspace_bytes(0, 4, 2, 64, 100) == 0
+
+
+def test_workspace_of_unknown_lengths():
+    """A bound of 0 means the same to the workspace's size as to the call: rows of any length."""
+    for rows, hq, hkv, d in ((1, 28, 4, 128), (3, 4, 2, 64), (9, 24, 1, 128), (300, 14, 2, 64)):
+        sizes = [K.paged_decode_attention_workspace_bytes(rows, hq, hkv, d, n) for n in (1, 600, 9000, 1 << 20, 1 << 30)]
+        assert sizes == sorted(sizes) and K.paged_decode_attention_workspace_bytes(rows, hq, hkv, d, 0) == sizes[-1]
