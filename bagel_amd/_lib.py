@@ -538,7 +538,7 @@ def paged_decode_attention(Q, cache: PagedCache, page_table, kv_lens, O, workspa
         _wrong_values(kv_lens, torch.int32, (rows,), "paged_decode_attention: kv_lens")
     if max_kv_len < 0:
         raise RuntimeError(f"paged_decode_attention: max_kv_len {max_kv_len}")
-    if softmax_scale is not None and (softmax_scale == 0 or not math.isfinite(softmax_scale)):
+    if softmax_scale is not None and not 0 < abs(F(softmax_scale).value) < math.inf:      # as the entry point gets it, in 32 bits
         raise RuntimeError(f"paged_decode_attention: softmax_scale {softmax_scale}")
     if not workspace.is_contiguous():
         raise RuntimeError("paged_decode_attention: contiguous workspace expected")

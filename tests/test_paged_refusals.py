@@ -150,3 +150,10 @@ def test_workspace_of_unknown_lengths():
     for rows, hq, hkv, d in ((1, 28, 4, 128), (3, 4, 2, 64), (9, 24, 1, 128), (300, 14, 2, 64)):
         sizes = [K.paged_decode_attention_workspace_bytes(rows, hq, hkv, d, n) for n in (1, 600, 9000, 1 << 20, 1 << 30)]
         assert sizes == sorted(sizes) and K.paged_decode_attention_workspace_bytes(rows, hq, hkv, d, 0) == sizes[-1]
+
+
+@pytest.mark.parametrize("scale", [1e-60, -1e-60, 1e300, -1e300])
+def test_attention_refuses_scales_that_32_bits_do_not_hold(scale):
+    """The entry point takes 32 bits, where these are 0 (which asks for 1 / sqrt(head_dim) instead) and infinity."""
+    with pytest.raises(RuntimeError, match="softmax_scale"):
+        _attend(softmax_scale=scale)
