@@ -201,7 +201,8 @@ class InterleaveInferencer:
                              max_think_token_n=1000, do_sample=False, text_temperature=0.3, cfg_text_scale=3.0,
                              cfg_img_scale=1.5, cfg_interval=[0.4, 1.0], timestep_shift=3.0, num_timesteps=50,
                              cfg_renorm_min=0.0, cfg_renorm_type="global", image_shapes=(1024, 1024),
-                             enable_taylorseer=False):
+                             enable_taylorseer=False, top_k=0, top_p=1.0, min_p=0.0, uniforms=None):
+        """top_k, top_p, min_p and uniforms are generate_text's, for the text that is decoded."""
         ctxs = CfgContexts(self)
         if think:
             ctxs.add_system_prompt(VLM_THINK_SYSTEM_PROMPT if understanding_output else GEN_THINK_SYSTEM_PROMPT)
@@ -215,7 +216,8 @@ class InterleaveInferencer:
             else:
                 raise ValueError(f"Unsupported input type: {type(term)}")
 
-        text_kwargs = dict(do_sample=do_sample, temperature=text_temperature, max_length=max_think_token_n)
+        text_kwargs = dict(do_sample=do_sample, temperature=text_temperature, max_length=max_think_token_n, top_k=top_k,
+                           top_p=top_p, min_p=min_p, uniforms=uniforms)
         if understanding_output:
             return [self.gen_text(ctxs.full, **text_kwargs)]
         outputs = []

@@ -43,3 +43,27 @@ def test_generate_text_refuses_settings_it_cannot_follow():
             model.generate_text(past_key_values=past, max_length=4, do_sample=True, **bad, **gi)
     with pytest.raises(ValueError):
         model.generate_text(past_key_values=past, max_length=4, uniforms=torch.rand(4, 1), **gi)
+
+
+def test_questions_take_the_filters():
+    """interleave_inference hands the sampling settings to the text it decodes."""
+    from bagel_amd.inferencer import InterleaveInferencer
+    from tests.test_gpu_text import _Tok
+    tc = TEXT_CASES["text_tiny_b1"]
+
+    class Tok(_Tok):
+        def decode(self, ids):
+            return "<|im_start|>" + " ".join(str(int(i)) for i in ids[1:]) + "<|im_end|>"
+
+    inf = InterleaveInferencer(_model(tc), None, Tok(), None, None, NEW_TOKEN_IDS)
+    prompt = " ".join(map(str, tc.prompts()[0]))
+    ctx = inf.update_context_text(prompt, inf.init_gen_context())
+    u = torch.rand((12, 1), generator=torch.Generator().manual_seed(5))
+    texts = []
+    for settings in (dict(top_k=20, top_p=0.8, uniforms=u), dict(min_p=0.05, uniforms=u), dict(uniforms=u), dict(top_k=1)):
+        want = inf.gen_text(ctx, max_length=12, do_sample=True, temperature=1.3, **settings)
+        assert inf.interleave_inference([prompt], understanding_output=True, do_sample=True, text_temperature=1.3, max_think_token_n=12,
+                                        **settings) == [want]
+        assert inf(text=prompt, understanding_output=True, do_sample=True, text_temperature=1.3, max_think_token_n=12, **settings)["text"] == want
+        texts.append(want)
+    assert texts[3] == inf.interleave_inference([prompt], understanding_output=True, do_sample=False, max_think_token_n=12)[0] != texts[2]
