@@ -168,10 +168,11 @@ int launch_append(const AppendParams& p, hipStream_t st) {
 // than one chunk is split over workgroups; each leaves an unnormalised partial (sums in fp32) and the last one to finish
 // joins them in chunk order, JOIN at a time: more chunks than that are joined in groups first.
 //
-// Bound by the reads of the cache.  28 query and 4 kv heads of 128: 64 rows of up to 8192 keys, 561 MB of bf16, 108 us =
-// 5.2 TB/s; one row of 131072, 268 MB, 55 us = 4.9 TB/s, joins included; e4m3, 200 rows of up to 4096, 476 MB, 93 us = 5.1 TB/s.
+// Bound by the reads of the cache.  28 query and 4 kv heads of 128: 64 rows of up to 8192 keys, 561 MB of bf16, 110 us =
+// 5.1 TB/s; one row of 131072, 268 MB, 55 us = 4.9 TB/s, joins included; e4m3, 200 rows of up to 4096, 476 MB, 94 us = 5.1 TB/s.
 // (Reads of random 16 KB pages alone reach 6.9 TB/s past the caches, 6.0 through them; a large copy 4.9.)
-// Keys straight to registers, 16 bytes of each of 16 rows per lane: 128 us for the first and 115 for the last of these.
+// Keys straight to registers, 16 bytes of each of 16 rows per lane, took 128 us for the first and 115 for the last of these where
+// keys through LDS took 108 and 93.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int WAVES = 4;
 constexpr int JOIN = 16;             // partials that are joined at once
@@ -621,6 +622,10 @@ Pool v_pool(const bagel_paged_cache* c) { return pool_of(c->v, c->v_page_stride,
 // per CU.  A level of joins takes 3 to 4 us, about as long as a workgroup takes for 512 keys: rows up to there are not split, and
 // rows of up to JOIN times as many into no more chunks than one level joins.  One row of 28 / 4 heads of 128 in bf16, so and with a
 // chunk per round: 500 keys 6.4 and 7.6 us, 3000 9.2 and 12.3, 8192 13.1 and 13.6 (four rows: 17.9 and 22.0).
+// Batches that fill the chip are not split, however long a row may be: max_kv_len is all that is known here, and a workgroup for a chunk
+// that its row turns out not to have takes 16 ns to come and go.  Chunks of at most 8192 keys in every batch bring 100 rows of 500
+// keys and one of 100000 from 1085 to 121 us, but 100 rows of 500 keys under a bound of 131072 from 26 to 133 us, and 1000 such rows from
+// 184 to 1224 us (at most 4096: 101, 230 and 2190; at most 16384: 186, 94 and 827).
 struct Split {
   int splits, chunk;
 };

@@ -18,7 +18,7 @@
 // slice's foremost tokens as (value, index) keys of 64 bits.  Bound by its vector instructions (busy 4/5 of the time), some
 // forty a logit and thread: 14 for bin and weight, 10 where tokens are listed, the rest once per slice.  A bin's count and weight
 // are the two parts of one 64-bit word, so that a logit is one LDS atomic.  Measured: 256 rows of 151936 32-bit logits, 156 MB,
-// 48 us = 3.3 TB/s; 64 rows of 152064 bf16 ones, 19 MB, 15.9 us; a single such row 6.6 us.
+// 48 us = 3.2 TB/s; 64 rows of 152064 bf16 ones, 19 MB, 15.8 us; a single such row 6.7 us.
 // The second (7 us for a row whose borders are listed, 30 us and more where borders lie deep in some rows): one workgroup per row, in one
 // of three ways:
 //   - a top-k of a few: the lists hold it, whatever the row's weights are, so the first launch only counted tokens (without weights),
