@@ -263,9 +263,9 @@ int bagel_paged_kv_append_bf16(const void* qkv, long ld, int rows, int Hq, const
  * pages hold, makes the outputs of that row (those of the kv heads that met it) NaN; nothing outside the pool is read.
  * max_kv_len: an upper bound of kv_lens (sizes the split over the length; 0 = unknown, table_width pages; a bound that is too small
  * costs time, not keys, and a wide one costs time too: 8 rows of 3000 keys of 28 / 4 heads of 128 take 15 us under their own length
- * and 67 us under 131072).  Rows are split while rows x kv heads are no more than the CUs; in larger batches one workgroup walks a
- * row's whole length, 11 us for 1000 bf16 keys of 128, so that a row far longer than the others is better off in a call of its own (100 rows of
- * 500 keys 26 us, one of 100000 alone 46 us, all in one call 1085 us).  softmax_scale 0: 1 / sqrt(head_dim).
+ * and 67 us under 131072).  Rows are split while rows x kv heads (x 16 query heads of each) are no more than the CUs; in larger
+ * batches one workgroup walks a row's whole length, 11 us for 1000 bf16 keys of 128, so that a row far longer than the others is better
+ * off in a call of its own (100 rows of 500 keys 26 us, one of 100000 alone 46 us, all in one call 1085 us).  softmax_scale 0: 1 / sqrt(head_dim).
  * workspace: bagel_paged_decode_attention_workspace_bytes(), which serves every call of this head layout with no more rows
  * and keys (max_kv_len 0: any number of keys); zero before the first call (the tickets at its start, which every call leaves zero);
  * calls that share one must not overlap, be they on two streams or in two replayed graphs.  rows <= 65535. */
